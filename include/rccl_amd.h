@@ -275,6 +275,107 @@ ncclResult_t rcclAmdAllReduceNoAlloc(const void* const* sendbuffs, void* const* 
  * nothing. */
 ncclResult_t rcclAmdNoAllocAsyncError(int device, ncclResult_t* asyncError);
 
+/* ---- local operators of a sharded training step ------------------------------------------------
+ * What a rank computes between a reduce-scatter and an all-gather: the optimizer step of its shard, and the sorting,
+ * dispatching and combining of token rows for the experts it holds.  Like rcclAmdReduceCopy they run on the current
+ * device, are enqueued on `stream`, allocate nothing, keep nothing from one call for the next, never wait for the GPU, and
+ * may be captured into a graph (a captured call keeps the pointers and host values that it was captured with).  Buffers
+ * are device memory of the current device; workspaces belong to the caller, must be 16-byte aligned and may not be shared
+ * by calls that can run at the same time.  Floating types: ncclFloat32, ncclBfloat16, ncclFloat16; every pointer has the
+ * alignment of its element type, no more is asked.  Outputs may not overlap inputs unless a call says so.  Results do not
+ * depend on the order in which the GPU runs things: the same call on the same data gives the same bits. */
+
+/* How AdamW's two moments are held.  rcclAmdStateF32: expAvg = m and expAvgSq = v as floats.
+ * rcclAmdStateMx8: expAvg holds m and expAvgSq holds sqrt(v) in OCP MX blocks: each 32 consecutive elements of a tensor
+ * (the last block may be shorter) are OCP e4m3 bytes (torch.float8_e4m3fn; not the encoding of ncclFp8E4M3) and share one
+ * scale byte X with the value 2^(X-127) in expAvgScale / expAvgSqScale.  All zero bytes are the initial state. */
+typedef enum { rcclAmdStateF32 = 0, rcclAmdStateMx8 = 1 } rcclAmdStateType_t;
+#define RCCL_AMD_STATE_BLOCK 32
+
+/* One tensor of a call: eight 8-byte words, so an array of them is also an n x 8 table of 64-bit integers. */
+typedef struct {
+  void* param;               /* read and written, paramType */
+  const void* grad;          /* gradType */
+  void* expAvg;              /* float, or e4m3 bytes */
+  void* expAvgSq;
+  uint8_t* expAvgScale;      /* rcclAmdStateMx8 only: ceil(count / 32) bytes each */
+  uint8_t* expAvgSqScale;
+  void* copy;                /* NULL, or where the updated parameter is written once more, rounded to copyType */
+  size_t count;              /* elements; 0 is allowed and does nothing */
+} rcclAmdAdamWTensor_t;
+
+typedef struct {
+  double lr, beta1, beta2, eps, weightDecay;
+  double gradScale;          /* gradients are multiplied by this first (1 / loss scale, 1 / ranks) */
+  double maxNorm;            /* with sumSq: gradients are scaled down to this norm where theirs is larger */
+  int64_t step;              /* 1 in the first step */
+  const int64_t* stepPtr;    /* device, or NULL: read by the kernel instead of `step` (for captured calls) */
+  const float* lrPtr;        /* device, or NULL: read by the kernel instead of `lr` */
+  const double* sumSq;       /* device, or NULL: no clipping.  The sum of squares of the unscaled gradients, of all ranks */
+  uint64_t seed;             /* rcclAmdStateMx8: of the random bits with which the moments are rounded */
+} rcclAmdAdamWConfig_t;
+
+/* AdamW over `ntensors` tensors, for each element (all of it in fp32):
+ *   c = gradScale * min(1, maxNorm / (gradScale * sqrt(*sumSq) + 1e-6))      (gradScale without sumSq)
+ *   g = c * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weightDecay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * param and copy are rounded to nearest.  Where *sumSq is not finite the step is skipped: parameters and states stay as
+ * they are and copy receives the unchanged parameter.
+ * An 8-bit state is rounded stochastically: a moving average with beta2 = 0.999 moves by less than half a step of an
+ * 8-bit float in an update, and rounding to nearest would leave it where it is.  The random bits are a hash of (seed,
+ * step, place of the tensor in the call, index of the element), so a step can be repeated exactly.  A sqrt(v) over zero is
+ * never rounded to zero.  copyType is ignored where every copy is NULL.  tensors is host memory, read before the call
+ * returns.  Tensors may not overlap one another. */
+ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntensors, ncclDataType_t paramType, ncclDataType_t gradType,
+                          ncclDataType_t copyType, rcclAmdStateType_t stateType, const rcclAmdAdamWConfig_t* config,
+                          hipStream_t stream);
+
+/* *out = (accumulate ? *out : 0) + the sum of the squares of all elements of `ntensors` tensors, in 64 bits (`out` is
+ * device memory).  An all-reduce of *out over the ranks is what rcclAmdAdamW takes as sumSq.  tensors and counts are host
+ * memory, read before the call returns.  The workspace holds rcclAmdSumSquaresBytes(ntensors) bytes. */
+ncclResult_t rcclAmdSumSquares(const void* const* tensors, const size_t* counts, int ntensors, ncclDataType_t datatype,
+                               double* out, int accumulate, void* workspace, size_t workspaceBytes, hipStream_t stream);
+ncclResult_t rcclAmdSumSquaresBytes(int ntensors, size_t* workspaceBytes);
+
+/* Sorts the tokens * topk slots of a router's choice by expert.  experts[t * topk + k] (ncclInt32 or ncclInt64) is the
+ * expert of slot t * topk + k; slots of the experts firstExpert .. firstExpert + nExperts - 1 are kept, all others (those
+ * of other ranks, -1 for padding) are dropped.  Expert e of the range gets the rows offsets[e] .. offsets[e] + counts[e] - 1
+ * in the order of the slots (the sort is stable), and offsets[e + 1] is the next multiple of rowAlign.
+ *   position[tokens * topk]   row of each slot, -1 where it is dropped
+ *   source[rows]              slot of each row, -1 for rows without one; rows = tokens * topk + nExperts * (rowAlign - 1)
+ *   offsets[nExperts + 1], counts[nExperts]
+ * source, offsets and counts may be NULL.  topk is 1 .. 64, nExperts 1 .. 1024, rowAlign 1 .. 1024, rows below 2^31.
+ * The workspace holds rcclAmdExpertSortBytes bytes (0: it may be NULL). */
+ncclResult_t rcclAmdExpertSort(const void* experts, ncclDataType_t expertType, size_t tokens, int topk, int64_t firstExpert,
+                               int nExperts, int rowAlign, int32_t* position, int32_t* source, int32_t* offsets,
+                               int32_t* counts, void* workspace, size_t workspaceBytes, hipStream_t stream);
+ncclResult_t rcclAmdExpertSortBytes(size_t tokens, int topk, int nExperts, size_t* workspaceBytes);
+
+/* Token rows in expert order: out[position[t * topk + k]] = x[t].  Rows of `hidden` elements, `xStride` and `outStride`
+ * elements apart; `out` has `rows` rows, and positions outside 0 .. rows - 1 are passed over.  With offsets and counts
+ * (both or neither, as rcclAmdExpertSort gives them) the padding rows offsets[e] + counts[e] .. offsets[e + 1] - 1 are set to
+ * zero; all other rows without a slot are left as they were.  Its gradient with respect to x is rcclAmdExpertCombine of
+ * the gradient of out, without weights. */
+ncclResult_t rcclAmdExpertDispatch(const void* x, size_t xStride, void* out, size_t outStride, size_t rows,
+                                   ncclDataType_t datatype, size_t tokens, int topk, size_t hidden, const int32_t* position,
+                                   const int32_t* offsets, const int32_t* counts, int nExperts, hipStream_t stream);
+
+/* Rows back in token order: y[t] = sum over k of weights[t * topk + k] * z[position[t * topk + k]], summed in fp32 in the
+ * order of k and rounded once.  weights NULL: all ones.  A token without a slot gets zeros.  z has `rows` rows. */
+ncclResult_t rcclAmdExpertCombine(const void* z, size_t zStride, size_t rows, const void* weights, ncclDataType_t weightType,
+                                  void* y, size_t yStride, ncclDataType_t datatype, size_t tokens, int topk, size_t hidden,
+                                  const int32_t* position, hipStream_t stream);
+
+/* The gradients of rcclAmdExpertCombine with weights: dz[position[t * topk + k]] = weights[t * topk + k] * dy[t] and
+ * dweights[t * topk + k] = the product of dy[t] with z[position[t * topk + k]] (weightType; zero where the slot is
+ * dropped).  Two slots may not name the same row.  Padding rows of dz as in rcclAmdExpertDispatch.  dz may be z itself,
+ * with the same stride. */
+ncclResult_t rcclAmdExpertCombineBackward(const void* dy, size_t dyStride, const void* z, size_t zStride, size_t rows,
+                                          const void* weights, ncclDataType_t weightType, void* dz, size_t dzStride,
+                                          void* dweights, ncclDataType_t datatype, size_t tokens, int topk, size_t hidden,
+                                          const int32_t* position, const int32_t* offsets, const int32_t* counts,
+                                          int nExperts, hipStream_t stream);
+
 /* Ring schedule synthesis for a single node whose GPUs are joined by direct xGMI links
  * (the job of the ring search + pre-baked models, src/graph/search.cc:919-986,
  * src/graph/rome_models.cc:549-560).  `adj` is an ngpus x ngpus 0/1 matrix of direct links.

@@ -1,0 +1,359 @@
+// AdamW over many tensors and the sum of squares that clips it: the local work of a rank between a reduce-scatter of
+// gradients and an all-gather of parameters.  Element-wise, bound by HBM: every element is read once and written once.
+#include <hip/hip_runtime.h>
+#include "local_ops.h"
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+// The same with the alignment of one element: tensors are views at any element of a flat buffer.  Unaligned vector
+// accesses are legal on gfx950, so one code path serves all of them.
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef f16x4 f16x4_u __attribute__((aligned(2)));
+typedef bf16x4 bf16x4_u __attribute__((aligned(2)));
+typedef uint32_t u32_u __attribute__((aligned(1)));
+
+template <typename T> struct Vec;
+template <> struct Vec<float> { typedef f32x4_u four; };
+template <> struct Vec<_Float16> { typedef f16x4_u four; };
+template <> struct Vec<__bf16> { typedef bf16x4_u four; };
+
+template <typename T> static __device__ __forceinline__ f32x4 load4(const T* p) {
+  return __builtin_convertvector(__builtin_nontemporal_load((const typename Vec<T>::four*)p), f32x4);
+}
+template <typename T> static __device__ __forceinline__ void store4(T* p, f32x4 x) {
+  typedef T vec __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store(__builtin_convertvector(x, vec), (typename Vec<T>::four*)p);
+}
+// `left` elements from p on exist (0 .. 4 of them are this lane's).
+template <typename T> static __device__ __forceinline__ f32x4 load4(const T* p, int left) {
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; i++) if (i < left) x[i] = (float)p[i];
+  return x;
+}
+template <typename T> static __device__ __forceinline__ void store4(T* p, f32x4 x, int left) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) if (i < left) p[i] = (T)x[i];
+}
+
+// 32 bits that depend on all of x: two rounds of xor-shift and multiplication by an odd constant (2^32 over the golden
+// ratio, and a multiplier of L'Ecuyer's tables of linear congruential generators).
+static __device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x = (x ^ (x >> 16)) * 0x9E3779B1u;
+  x = (x ^ (x >> 15)) * 0xAC564B05u;
+  return x ^ (x >> 16);
+}
+static __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+static __device__ __forceinline__ float uniform(float x) { return __uint_as_float(uniform(__float_as_uint(x))); }
+
+// Which of the launch's tensors chunk b belongs to: the number of tensors that begin at or before it, less one.
+static __device__ __forceinline__ uint32_t findTensor(const uint32_t* first, uint32_t n, uint32_t b) {
+  uint32_t t = 0;
+  for (uint32_t k = 0; k < n; k += 64) {
+    const uint32_t i = k + (threadIdx.x & 63);
+    t += (uint32_t)__popcll(__ballot(i < n && first[i < n ? i : 0] <= b));
+  }
+  return uniform(t - 1);
+}
+
+// x^n by squaring, in 64 bits; the host computes its bias corrections with the same steps.
+static __device__ __forceinline__ double powN(double x, int64_t n) {
+  double r = 1.0;
+  for (; n > 0; n >>= 1, x *= x) if (n & 1) r *= x;
+  return r;
+}
+
+struct Scalars { float b1, omb1, b2, omb2, eps, decay, stepSize, rootC2, coef; };
+
+// ------------------------------------------------------------------ 8-bit states
+static __device__ __forceinline__ f32x4 decode4(uint32_t code, uint32_t scale) {
+  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, true);
+  const float f = __uint_as_float(scale << 23);          // 2^(X-127); 0 for X = 0, which only an all-zero block has
+  return f32x4{lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f};
+}
+static __device__ __forceinline__ uint32_t maxOf8(uint32_t a) {      // over the 8 lanes that hold a block, with DPP moves
+  uint32_t o;
+  o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0xB1, 0xF, 0xF, true); a = a > o ? a : o;      // lane ^ 1
+  o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x4E, 0xF, 0xF, true); a = a > o ? a : o;      // lane ^ 2
+  o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x141, 0xF, 0xF, true); return a > o ? a : o;  // 7 - lane
+}
+// The scale of a block: the smallest power of two with which its largest magnitude (bit pattern `most`) is at most 448.
+static __device__ __forceinline__ uint32_t scaleOf(uint32_t most) {
+  const int x = (int)((most + 0x1FFFFFu) >> 23) - 8;
+  return (uint32_t)(x < 1 ? 1 : x > 247 ? 247 : x);
+}
+// Stochastic rounding to the e4m3 grid.  y is the scaled value, rnd 20 random bits: they are added below the third bit of
+// the mantissa and what is below it is cut off.  Values under 2^-6 are moved to the binade above first, whose grid of 2^-9
+// is that of e4m3's subnormal numbers.  The result is a value of the grid, so the conversion that follows is exact.
+template <bool KEEP> static __device__ __forceinline__ float roundRandom(float y, uint32_t rnd) {
+  const float a = __builtin_fabsf(y);
+  const float low = a < 0x1p-6f ? 0x1p-6f : 0.f;
+  float c = __uint_as_float((__float_as_uint(a + low) + rnd) & 0xFFF00000u) - low;
+  if (KEEP && y > 0.f) c = c > 0x1p-9f ? c : 0x1p-9f;    // a second moment over zero stays over zero
+  c = __builtin_copysignf(c, y);
+  return a < __builtin_inff() ? c : __builtin_nanf("");
+}
+template <bool KEEP> static __device__ __forceinline__ uint32_t encode4(f32x4 x, uint32_t scale, const uint32_t (&rnd)[4]) {
+  const float inv = __uint_as_float((254u - scale) << 23);
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) y[i] = roundRandom<KEEP>(x[i] * inv, rnd[i]);
+  int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
+}
+static __device__ __forceinline__ uint32_t bitsMax(f32x4 x) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) { const uint32_t b = __float_as_uint(x[i]) & 0x7FFFFFFFu; a = a > b ? a : b; }
+  return a;
+}
+
+// ------------------------------------------------------------------ AdamW
+// A workgroup of four waves takes one chunk of one tensor; a wave takes rows of 256 elements, 4 for each lane, so that
+// every access of a row is one contiguous run and a block of an 8-bit state lies in 8 neighbouring lanes.
+template <typename P, typename G, bool MX> struct Row {
+  P* param; const G* grad;
+  float *m, *v;                         // fp32 states
+  uint8_t *cm, *cv, *sm, *sv;           // 8-bit states
+  void* copy; int copyType;
+  f32x4 p, g, fm, fv;
+  uint32_t qm, qv, xm, xv;
+
+  template <bool FULL> __device__ __forceinline__ void load(size_t at, int left) {
+    if (FULL) { p = load4(param + at); g = load4(grad + at); }
+    else { p = load4(param + at, left); g = load4(grad + at, left); }
+    if constexpr (MX) {
+      if (FULL) { qm = __builtin_nontemporal_load((const u32_u*)(cm + at)); qv = __builtin_nontemporal_load((const u32_u*)(cv + at)); }
+      else {
+        qm = qv = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) if (i < left) { qm |= (uint32_t)cm[at + i] << (8 * i); qv |= (uint32_t)cv[at + i] << (8 * i); }
+      }
+      xm = xv = 0;
+      if (FULL || left > 0) { xm = sm[at / RCCL_AMD_STATE_BLOCK]; xv = sv[at / RCCL_AMD_STATE_BLOCK]; }
+    } else if (FULL) { fm = load4(m + at); fv = load4(v + at); }
+    else { fm = load4(m + at, left); fv = load4(v + at, left); }
+  }
+  template <bool FULL> __device__ __forceinline__ void storeCopy(size_t at, int left) {
+    if (copyType < 0) return;
+    if (copyType == ncclFloat32) { if (FULL) store4((float*)copy + at, p); else store4((float*)copy + at, p, left); }
+    else if (copyType == ncclBfloat16) { if (FULL) store4((__bf16*)copy + at, p); else store4((__bf16*)copy + at, p, left); }
+    else { if (FULL) store4((_Float16*)copy + at, p); else store4((_Float16*)copy + at, p, left); }
+  }
+  // Division and square root are the correctly rounded ones; nothing is contracted, so that a rounding of an 8-bit state
+  // does not depend on how this is compiled.
+  template <bool FULL> __device__ __forceinline__ void update(const Scalars& s, size_t at, int left, uint32_t key) {
+    f32x4 r;
+    if constexpr (MX) { fm = decode4(qm, xm); r = decode4(qv, xv); fv = r * r; }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float gi = g[i] * s.coef;
+      fm[i] = s.b1 * fm[i] + s.omb1 * gi;
+      fv[i] = s.b2 * fv[i] + s.omb2 * (gi * gi);
+      r[i] = __builtin_sqrtf(fv[i]);
+      p[i] = p[i] * s.decay - s.stepSize * (fm[i] / (r[i] * s.rootC2 + s.eps));
+    }
+    if (FULL) store4(param + at, p); else store4(param + at, p, left);
+    storeCopy<FULL>(at, left);
+    if constexpr (MX) {
+      if (!FULL) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) if (i >= left) { fm[i] = 0.f; r[i] = 0.f; }
+      }
+      const uint32_t em = scaleOf(maxOf8(bitsMax(fm))), ev = scaleOf(maxOf8(bitsMax(r)));
+      uint32_t rm[4], rv[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t h = mix((uint32_t)at + (uint32_t)i + key);
+        rm[i] = (h & 0xFFFFu) << 4 | 8u;
+        rv[i] = (h >> 16) << 4 | 8u;
+      }
+      const uint32_t nm = encode4<false>(fm, em, rm), nv = encode4<true>(r, ev, rv);
+      if (FULL) { __builtin_nontemporal_store(nm, (u32_u*)(cm + at)); __builtin_nontemporal_store(nv, (u32_u*)(cv + at)); }
+      else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) if (i < left) { cm[at + i] = (uint8_t)(nm >> (8 * i)); cv[at + i] = (uint8_t)(nv >> (8 * i)); }
+      }
+      if ((threadIdx.x & 7) == 0 && (FULL || left > 0)) { sm[at / RCCL_AMD_STATE_BLOCK] = (uint8_t)em; sv[at / RCCL_AMD_STATE_BLOCK] = (uint8_t)ev; }
+    } else if (FULL) { store4(m + at, fm); store4(v + at, fv); }
+    else { store4(m + at, fm, left); store4(v + at, fv, left); }
+  }
+};
+
+template <typename P, typename G, bool MX>
+__global__ __launch_bounds__(RA_ADAMW_THREADS) void raLocalKernelAdamW(RaAdamWArgs a) {
+  constexpr int U = 2;                                      // rows in flight for each wave
+  constexpr uint32_t STEP = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW;
+  const uint32_t t = findTensor(a.first, a.n, blockIdx.x);
+  const uint64_t* w = a.words + (size_t)t * a.stride;
+  const size_t count = w[RA_W_COUNT];
+  const size_t begin = (size_t)(blockIdx.x - a.first[t]) * a.chunk;
+  const size_t end = begin + a.chunk < count ? begin + a.chunk : count;
+
+  Scalars s = {a.b1, a.omb1, a.b2, a.omb2, a.eps, a.decay, a.stepSize, a.rootC2, a.coef};
+  int64_t step = a.step;
+  if (a.stepPtr || a.lrPtr) {
+    if (a.stepPtr) step = *a.stepPtr;
+    const double lr = a.lrPtr ? (double)*a.lrPtr : a.lr;
+    s.decay = uniform((float)(1.0 - lr * a.weightDecay));
+    s.stepSize = uniform((float)(lr / (1.0 - powN(a.beta1, step))));
+    s.rootC2 = uniform((float)(1.0 / __builtin_sqrt(1.0 - powN(a.beta2, step))));
+  }
+  bool go = true;
+  if (a.sumSq) {
+    const double sq = *a.sumSq;
+    go = __builtin_isfinite(sq);
+    const double c = a.maxNorm / (a.gradScale * __builtin_sqrt(sq) + 1e-6);
+    s.coef = uniform((float)(a.gradScale * (c < 1.0 ? c : 1.0)));
+  }
+
+  Row<P, G, MX> row[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    row[u].param = (P*)w[RA_W_PARAM]; row[u].grad = (const G*)w[RA_W_GRAD];
+    if constexpr (MX) { row[u].cm = (uint8_t*)w[RA_W_M]; row[u].cv = (uint8_t*)w[RA_W_V]; row[u].sm = (uint8_t*)w[RA_W_MS]; row[u].sv = (uint8_t*)w[RA_W_VS]; }
+    else { row[u].m = (float*)w[RA_W_M]; row[u].v = (float*)w[RA_W_V]; }
+    row[u].copy = a.copyWord >= 0 ? (void*)w[a.copyWord] : nullptr;
+    row[u].copyType = row[u].copy ? a.copyType : -1;
+  }
+  const uint32_t lane4 = (threadIdx.x & 63) * 4;
+  size_t r = begin + uniform(threadIdx.x >> 6) * RA_ADAMW_ROW;
+  if (!go) {                                                // a skipped step: only the copies are written
+    if (row[0].copyType >= 0)
+      for (; r < end; r += STEP) {
+        const size_t at = r + lane4;
+        const int left = at < end ? (end - at < 4 ? (int)(end - at) : 4) : 0;
+        row[0].p = load4(row[0].param + at, left);
+        row[0].template storeCopy<false>(at, left);
+      }
+    return;
+  }
+  uint32_t key = 0;
+  if constexpr (MX) {
+    key = mix((uint32_t)a.seed + 0x9E3779B9u);
+    key = mix(key ^ (uint32_t)(a.seed >> 32));
+    key = mix(key + (uint32_t)step);
+    key = uniform(mix(a.ordinal + t + key));
+  }
+  for (; r + (U - 1) * STEP + RA_ADAMW_ROW <= end; r += U * STEP) {
+#pragma unroll
+    for (int u = 0; u < U; u++) row[u].template load<true>(r + u * STEP + lane4, 4);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const size_t at = r + u * STEP;
+      const uint32_t k = at >> 32 ? mix(key ^ (uint32_t)(at >> 32)) : key;
+      row[u].template update<true>(s, at + lane4, 4, k);
+    }
+  }
+  for (; r < end; r += STEP) {
+    const size_t at = r + lane4;
+    const uint32_t k = r >> 32 ? mix(key ^ (uint32_t)(r >> 32)) : key;
+    if (r + RA_ADAMW_ROW <= end) {
+      row[0].template load<true>(at, 4);
+      row[0].template update<true>(s, at, 4, k);
+    } else {
+      const int left = at < end ? (end - at < 4 ? (int)(end - at) : 4) : 0;
+      row[0].template load<false>(at, left);
+      row[0].template update<false>(s, at, left, k);
+    }
+  }
+}
+
+template <typename P, typename G>
+static hipError_t adamW(const RaAdamWArgs& a, bool mx, uint32_t grid, hipStream_t s) {
+  if (mx) hipLaunchKernelGGL((raLocalKernelAdamW<P, G, true>), dim3(grid), dim3(RA_ADAMW_THREADS), 0, s, a);
+  else hipLaunchKernelGGL((raLocalKernelAdamW<P, G, false>), dim3(grid), dim3(RA_ADAMW_THREADS), 0, s, a);
+  return hipGetLastError();
+}
+template <typename P>
+static hipError_t adamWGrad(const RaAdamWArgs& a, int gradType, bool mx, uint32_t grid, hipStream_t s) {
+  switch (gradType) {
+    case ncclFloat32: return adamW<P, float>(a, mx, grid, s);
+    case ncclBfloat16: return adamW<P, __bf16>(a, mx, grid, s);
+    case ncclFloat16: return adamW<P, _Float16>(a, mx, grid, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+hipError_t raLaunchAdamW(const RaAdamWArgs& a, int paramType, int gradType, bool mx, uint32_t grid, hipStream_t s) {
+  switch (paramType) {
+    case ncclFloat32: return adamWGrad<float>(a, gradType, mx, grid, s);
+    case ncclBfloat16: return adamWGrad<__bf16>(a, gradType, mx, grid, s);
+    case ncclFloat16: return adamWGrad<_Float16>(a, gradType, mx, grid, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+// ------------------------------------------------------------------ sum of squares
+// One partial sum for each chunk, in 64 bits, then one workgroup that adds the partial sums in a fixed order: the result
+// does not depend on which chunk is done first.  Squares of fp32 values overflow fp32 long before their norm does, so
+// the products are 64-bit too.
+static __device__ __forceinline__ double waveSum(double x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+  return x;
+}
+template <int THREADS> static __device__ __forceinline__ double blockSum(double x) {      // valid in thread 0
+  __shared__ double sums[THREADS / 64];
+  x = waveSum(x);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = 0.0;
+  if (threadIdx.x == 0) for (int i = 0; i < THREADS / 64; i++) x += sums[i];
+  return x;
+}
+template <typename T> static __device__ __forceinline__ f32x4 load4Cached(const T* p) {   // AdamW reads the gradients next
+  return __builtin_convertvector(*(const typename Vec<T>::four*)p, f32x4);
+}
+template <typename T>
+__global__ __launch_bounds__(RA_SUMSQ_THREADS) void raLocalKernelSumSq(RaSumSqArgs a) {
+  const uint32_t t = findTensor(a.first, a.n, blockIdx.x);
+  const T* x = (const T*)a.ptr[t];
+  const uint32_t count = a.count[t];
+  const uint64_t begin = (uint64_t)(blockIdx.x - a.first[t]) * a.chunk;
+  const uint64_t end = begin + a.chunk < count ? begin + a.chunk : count;
+  constexpr int U = 4;
+  constexpr uint32_t STEP = RA_SUMSQ_THREADS * 4;
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+  uint64_t r = begin + threadIdx.x * 4;
+  for (; r + (U - 1) * STEP + 4 <= end; r += U * STEP) {
+    f32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) v[u] = load4Cached(x + r + u * STEP);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) sum[i] = __builtin_fma((double)v[u][i], (double)v[u][i], sum[i]);
+  }
+  for (; r < end; r += STEP) {
+    const f32x4 v = load4(x + r, end - r < 4 ? (int)(end - r) : 4);
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum[i] = __builtin_fma((double)v[i], (double)v[i], sum[i]);
+  }
+  const double all = blockSum<RA_SUMSQ_THREADS>((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if (threadIdx.x == 0) {
+    if (a.out) *a.out = (a.accumulate ? *a.out : 0.0) + all;
+    else a.partial[blockIdx.x] = all;
+  }
+}
+__global__ __launch_bounds__(1024) void raLocalKernelSumSqJoin(const double* __restrict__ partial, uint32_t n, double* out, int accumulate) {
+  double sum = 0.0;
+  for (uint32_t i = threadIdx.x; i < n; i += 1024) sum += partial[i];
+  sum = blockSum<1024>(sum);
+  if (threadIdx.x == 0) *out = (accumulate ? *out : 0.0) + sum;
+}
+
+hipError_t raLaunchSumSq(const RaSumSqArgs& a, int type, uint32_t grid, hipStream_t s) {
+  switch (type) {
+    case ncclFloat32: hipLaunchKernelGGL((raLocalKernelSumSq<float>), dim3(grid), dim3(RA_SUMSQ_THREADS), 0, s, a); break;
+    case ncclBfloat16: hipLaunchKernelGGL((raLocalKernelSumSq<__bf16>), dim3(grid), dim3(RA_SUMSQ_THREADS), 0, s, a); break;
+    case ncclFloat16: hipLaunchKernelGGL((raLocalKernelSumSq<_Float16>), dim3(grid), dim3(RA_SUMSQ_THREADS), 0, s, a); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+hipError_t raLaunchSumSqJoin(const double* partial, uint32_t n, double* out, int accumulate, hipStream_t s) {
+  hipLaunchKernelGGL(raLocalKernelSumSqJoin, dim3(1), dim3(1024), 0, s, partial, n, out, accumulate);
+  return hipGetLastError();
+}

@@ -22,6 +22,9 @@ ncclFloat16, ncclFloat32, ncclFloat64, ncclBfloat16, ncclFp8E4M3, ncclFp8E5M2 = 
 ncclChar, ncclInt, ncclHalf, ncclFloat, ncclDouble = ncclInt8, ncclInt32, ncclFloat16, ncclFloat32, ncclFloat64
 ncclScalarDevice, ncclScalarHostImmediate = 0, 1
 NCCL_UNIQUE_ID_BYTES = 128
+# rcclAmdStateType_t: how AdamW's moments are held
+rcclAmdStateF32, rcclAmdStateMx8 = 0, 1
+STATE_BLOCK = 32                    # elements of an 8-bit state that share a scale byte
 
 TYPE_SIZE = {ncclInt8: 1, ncclUint8: 1, ncclInt32: 4, ncclUint32: 4, ncclInt64: 8, ncclUint64: 8,
              ncclFloat16: 2, ncclFloat32: 4, ncclFloat64: 8, ncclBfloat16: 2, ncclFp8E4M3: 1, ncclFp8E5M2: 1}
@@ -37,6 +40,8 @@ EXPORTS = [
     "mscclUnloadAlgo", "rcclAmdReduceCopy", "rcclAmdTopoRings", "rcclAmdTopoParseXml", "rcclAmdPlanInfo",
     "rcclAmdPlanForConfig", "rcclAmdPlanProtoForConfig", "rcclAmdBootstrapAllGather", "rcclAmdAllReduceNoAlloc",
     "rcclAmdNoAllocAsyncError", "rcclAmdTopoFromLinks", "rcclAmdWindowBytesFor",
+    "rcclAmdAdamW", "rcclAmdSumSquares", "rcclAmdSumSquaresBytes", "rcclAmdExpertSort", "rcclAmdExpertSortBytes",
+    "rcclAmdExpertDispatch", "rcclAmdExpertCombine", "rcclAmdExpertCombineBackward",
 ]
 EXPORTS += ["p" + name for name in EXPORTS if name.startswith(("nccl", "msccl"))]      # profiling aliases
 
@@ -51,11 +56,22 @@ class ncclConfig_t(ctypes.Structure):
                 ("maxCTAs", ctypes.c_int), ("netName", ctypes.c_char_p), ("splitShare", ctypes.c_int)]
 
 
+class rcclAmdAdamWTensor_t(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("expAvg", ctypes.c_void_p), ("expAvgSq", ctypes.c_void_p),
+                ("expAvgScale", ctypes.c_void_p), ("expAvgSqScale", ctypes.c_void_p), ("copy", ctypes.c_void_p), ("count", ctypes.c_size_t)]
+
+
+class rcclAmdAdamWConfig_t(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weightDecay", ctypes.c_double), ("gradScale", ctypes.c_double), ("maxNorm", ctypes.c_double), ("step", ctypes.c_int64),
+                ("stepPtr", ctypes.c_void_p), ("lrPtr", ctypes.c_void_p), ("sumSq", ctypes.c_void_p), ("seed", ctypes.c_uint64)]
+
+
 class NcclError(RuntimeError):
-    def __init__(self, code, where):
+    def __init__(self, code, where, last=None):
         self.code = code
         msg = lib().ncclGetErrorString(code).decode()
-        last = lib().ncclGetLastError(None).decode()
+        last = lib().ncclGetLastError(None).decode() if last is None else last
         super().__init__(f"{where}: {msg} [{code}] {last}")
 
 
@@ -118,6 +134,14 @@ def lib():
         L.rcclAmdNoAllocAsyncError.argtypes = [ci, ctypes.POINTER(ci)]
         L.rcclAmdTopoFromLinks.argtypes = [ci, ctypes.POINTER(ctypes.c_uint), ctypes.POINTER(ctypes.c_uint), ctypes.POINTER(ci), ctypes.POINTER(ci)]
         L.rcclAmdWindowBytesFor.argtypes = [ci, ci, ctypes.POINTER(sz), ctypes.POINTER(sz), ctypes.POINTER(sz), ctypes.POINTER(ci)]
+        L.rcclAmdAdamW.argtypes = [vp, ci, ci, ci, ci, ci, ctypes.POINTER(rcclAmdAdamWConfig_t), vp]
+        L.rcclAmdSumSquares.argtypes = [vp, vp, ci, ci, vp, ci, vp, sz, vp]
+        L.rcclAmdSumSquaresBytes.argtypes = [ci, ctypes.POINTER(sz)]
+        L.rcclAmdExpertSort.argtypes = [vp, ci, sz, ci, ctypes.c_int64, ci, ci, vp, vp, vp, vp, vp, sz, vp]
+        L.rcclAmdExpertSortBytes.argtypes = [sz, ci, ci, ctypes.POINTER(sz)]
+        L.rcclAmdExpertDispatch.argtypes = [vp, sz, vp, sz, sz, ci, sz, ci, sz, vp, vp, vp, ci, vp]
+        L.rcclAmdExpertCombine.argtypes = [vp, sz, sz, vp, ci, vp, sz, ci, sz, ci, sz, vp, vp]
+        L.rcclAmdExpertCombineBackward.argtypes = [vp, sz, vp, sz, sz, vp, ci, vp, sz, vp, ci, sz, ci, sz, vp, vp, vp, ci, vp]
         _lib = L
     return _lib
 
@@ -351,6 +375,191 @@ def reduce_copy(dst, srcs, count, datatype, op=ncclSum, stream=None):
     arr = (ctypes.c_void_p * len(srcs))(*[_ptr(s).value for s in srcs])
     _check(lib().rcclAmdReduceCopy(_ptr(dst), arr, len(srcs), count, datatype, op, _stream(stream)),
            "rcclAmdReduceCopy")
+
+
+# ---- local operators of a sharded training step (see include/rccl_amd.h for the formulas) ----------------------------
+# A buffer is a device pointer (int) or a torch tensor.  A tensor is checked before its address is taken: on the current
+# device, of the element type the call names, and reaching as far as the call will.  Rows may be strided: the stride of a
+# two-dimensional tensor is taken from it.
+
+_TORCH_TYPES = {}
+
+
+def _torch_types():
+    if not _TORCH_TYPES:
+        import torch
+        _TORCH_TYPES.update({ncclFloat32: torch.float32, ncclBfloat16: torch.bfloat16, ncclFloat16: torch.float16, ncclFloat64: torch.float64,
+                             ncclInt32: torch.int32, ncclInt64: torch.int64, "current": torch.cuda.current_device})
+    return _TORCH_TYPES
+
+
+def _refuse(where, why):
+    raise NcclError(ncclInvalidArgument, where, why)
+
+
+def _whole(x, n, datatype, where, name):
+    """Address of `n` contiguous elements of `datatype`."""
+    if x is None or isinstance(x, int):
+        return x
+    t = _torch_types()
+    if not x.is_cuda or x.device.index != t["current"]():
+        _refuse(where, f"{name} is on {x.device}, not on the current device")
+    if x.dtype != t[datatype]:
+        _refuse(where, f"{name} is {x.dtype}, the call names type {datatype}")
+    if x.numel() < n or not x.is_contiguous():
+        _refuse(where, f"{name} has {x.numel()} elements ({'' if x.is_contiguous() else 'not '}contiguous), {n} are needed")
+    return x.data_ptr()
+
+
+def _matrix(x, stride, rows, hidden, datatype, where, name):
+    """(address, stride) of `rows` rows of `hidden` elements of `datatype`, each row contiguous."""
+    if x is None or isinstance(x, int):
+        return x, hidden if stride is None else stride
+    t = _torch_types()
+    if not x.is_cuda or x.device.index != t["current"]():
+        _refuse(where, f"{name} is on {x.device}, not on the current device")
+    if x.dtype != t[datatype]:
+        _refuse(where, f"{name} is {x.dtype}, the call names type {datatype}")
+    shape = x.shape
+    if len(shape) != 2 or shape[0] < rows or shape[1] < hidden or (shape[1] > 1 and x.stride(1) != 1):
+        _refuse(where, f"{name} has shape {tuple(shape)} and strides {x.stride()}, {rows} contiguous rows of {hidden} are needed")
+    own = x.stride(0) if shape[0] > 1 else max(hidden, x.stride(0))
+    if stride is not None and stride != own:
+        _refuse(where, f"{name} has a row stride of {own}, the call names {stride}")
+    return x.data_ptr(), own
+
+
+def _work(x, nbytes, where):
+    if x is None or isinstance(x, int):
+        return x, nbytes
+    if not x.is_cuda or x.device.index != _torch_types()["current"]():
+        _refuse(where, f"the workspace is on {x.device}, not on the current device")
+    if not x.is_contiguous():
+        _refuse(where, "the workspace is not contiguous")
+    return x.data_ptr(), x.numel() * x.element_size()
+
+
+def _host_table(x, columns, where):
+    """(address, rows, what keeps it alive) of a C-contiguous host array of 8-byte integers."""
+    import numpy as np
+    a = np.ascontiguousarray(x)
+    if a.dtype.kind not in "iu" or a.dtype.itemsize != 8:
+        if a.size and a.dtype.kind not in "iu":
+            _refuse(where, f"a table of 64-bit integers is needed, got {a.dtype}")
+        a = a.astype(np.int64)
+    if a.ndim != (1 if columns is None else 2) or (columns is not None and a.shape[1] != columns):
+        _refuse(where, f"a table of shape {a.shape}")
+    return a.ctypes.data, a.shape[0], a
+
+
+def adamw_tensor(param, grad, exp_avg, exp_avg_sq, count=None, exp_avg_scale=None, exp_avg_sq_scale=None, copy=None):
+    """One row of the table that adamw() takes, from contiguous tensors or device pointers (then with `count`)."""
+    tensors = [x for x in (param, grad, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, copy) if x is not None and not isinstance(x, int)]
+    if count is None:
+        if isinstance(param, int):
+            _refuse("adamw_tensor", "a device pointer needs a count")
+        count = param.numel()
+    blocks = -(-count // STATE_BLOCK)
+    for x in tensors:
+        if not x.is_cuda or x.device.index != _torch_types()["current"]() or not x.is_contiguous():
+            _refuse("adamw_tensor", f"a tensor on {x.device} with strides {x.stride()}: contiguous ones on the current device are needed")
+        if x.numel() < (blocks if x is exp_avg_scale or x is exp_avg_sq_scale else count):
+            _refuse("adamw_tensor", f"a tensor of {x.numel()} elements for a parameter of {count}")
+    at = lambda x: 0 if x is None else x if isinstance(x, int) else x.data_ptr()  # noqa: E731
+    return [at(param), at(grad), at(exp_avg), at(exp_avg_sq), at(exp_avg_scale), at(exp_avg_sq_scale), at(copy), count]
+
+
+def adamw(tensors, param_type, grad_type, copy_type=-1, state_type=rcclAmdStateF32, *, lr, beta1=0.9, beta2=0.999, eps=1e-8,
+          weight_decay=0.01, step=1, step_ptr=None, lr_ptr=None, grad_scale=1.0, sum_sq=None, max_norm=0.0, seed=0, stream=None):
+    """rcclAmdAdamW.  `tensors`: an (n, 8) table of 64-bit integers, one row for each tensor as adamw_tensor() gives it
+    (the fields of rcclAmdAdamWTensor_t); a program whose buffers stay where they are keeps the table.  step_ptr (int64),
+    lr_ptr (float32) and sum_sq (float64) are one-element device buffers that the kernel reads."""
+    where = "rcclAmdAdamW"
+    rows, n, keep = _host_table(tensors, 8, where) if len(tensors) else (None, 0, None)
+    c = rcclAmdAdamWConfig_t(lr, beta1, beta2, eps, weight_decay, grad_scale, max_norm, step, _whole(step_ptr, 1, ncclInt64, where, "step_ptr"),
+                             _whole(lr_ptr, 1, ncclFloat32, where, "lr_ptr"), _whole(sum_sq, 1, ncclFloat64, where, "sum_sq"), seed & 0xFFFFFFFFFFFFFFFF)
+    _check(lib().rcclAmdAdamW(rows, n, param_type, grad_type, copy_type, state_type, ctypes.byref(c), _stream(stream)), where)
+    del keep
+
+
+def sum_squares_bytes(n):
+    """rcclAmdSumSquaresBytes: bytes of workspace for `n` tensors."""
+    v = ctypes.c_size_t()
+    _check(lib().rcclAmdSumSquaresBytes(n, ctypes.byref(v)), "rcclAmdSumSquaresBytes")
+    return v.value
+
+
+def sum_squares(tensors, counts, datatype, out, workspace, accumulate=False, stream=None):
+    """rcclAmdSumSquares: out[0] (float64) = sum of the squares of all elements.  `tensors`: a list of torch tensors (counts
+    may be None) or an array of device addresses, `counts` an array of their sizes."""
+    where = "rcclAmdSumSquares"
+    if len(tensors) and not isinstance(tensors[0], int) and hasattr(tensors[0], "data_ptr"):
+        counts = [t.numel() for t in tensors] if counts is None else counts
+        tensors = [_whole(t, n, datatype, where, "a tensor") for t, n in zip(tensors, counts)]
+    if counts is None or len(counts) != len(tensors):
+        _refuse(where, f"{len(tensors)} tensors with other counts")
+    ptrs, n, keep = _host_table(tensors, None, where) if len(tensors) else (None, 0, None)
+    sizes, _, keep2 = _host_table(counts, None, where) if len(tensors) else (None, 0, None)
+    w, nbytes = _work(workspace, sum_squares_bytes(n), where)
+    _check(lib().rcclAmdSumSquares(ptrs, sizes, n, datatype, _whole(out, 1, ncclFloat64, where, "out"), int(accumulate), w, nbytes, _stream(stream)), where)
+    del keep, keep2
+
+
+def expert_rows(tokens, topk, n_experts, row_align=1):
+    """Rows of the sorted order: every slot, and up to row_align - 1 rows of padding for each expert."""
+    return tokens * topk + n_experts * (row_align - 1)
+
+
+def expert_sort_bytes(tokens, topk, n_experts):
+    """rcclAmdExpertSortBytes: bytes of workspace of expert_sort."""
+    v = ctypes.c_size_t()
+    _check(lib().rcclAmdExpertSortBytes(tokens, topk, n_experts, ctypes.byref(v)), "rcclAmdExpertSortBytes")
+    return v.value
+
+
+def expert_sort(experts, expert_type, tokens, topk, first_expert, n_experts, row_align, position, source=None, offsets=None, counts=None,
+                workspace=None, stream=None):
+    """rcclAmdExpertSort: rows of the slots in the order of the experts first_expert .. first_expert + n_experts - 1."""
+    where = "rcclAmdExpertSort"
+    slots = tokens * topk
+    w, nbytes = _work(workspace, 0, where) if workspace is None or not isinstance(workspace, int) else (workspace, expert_sort_bytes(tokens, topk, n_experts))
+    _check(lib().rcclAmdExpertSort(_whole(experts, slots, expert_type, where, "experts"), expert_type, tokens, topk, first_expert, n_experts, row_align,
+                                   _whole(position, slots, ncclInt32, where, "position"),
+                                   _whole(source, expert_rows(tokens, topk, n_experts, row_align), ncclInt32, where, "source"),
+                                   _whole(offsets, n_experts + 1, ncclInt32, where, "offsets"), _whole(counts, n_experts, ncclInt32, where, "counts"),
+                                   w, nbytes, _stream(stream)), where)
+
+
+def expert_dispatch(x, out, rows, datatype, tokens, topk, hidden, position, offsets=None, counts=None, n_experts=0, x_stride=None, out_stride=None, stream=None):
+    """rcclAmdExpertDispatch: out[position[t, k]] = x[t]; its gradient is expert_combine of out's without weights."""
+    where = "rcclAmdExpertDispatch"
+    x, xs = _matrix(x, x_stride, tokens, hidden, datatype, where, "x")
+    out, os_ = _matrix(out, out_stride, rows, hidden, datatype, where, "out")
+    _check(lib().rcclAmdExpertDispatch(x, xs, out, os_, rows, datatype, tokens, topk, hidden, _whole(position, tokens * topk, ncclInt32, where, "position"),
+                                       _whole(offsets, n_experts + 1, ncclInt32, where, "offsets"), _whole(counts, n_experts, ncclInt32, where, "counts"),
+                                       n_experts, _stream(stream)), where)
+
+
+def expert_combine(z, rows, weights, weight_type, y, datatype, tokens, topk, hidden, position, z_stride=None, y_stride=None, stream=None):
+    """rcclAmdExpertCombine: y[t] = sum over k of weights[t, k] * z[position[t, k]]; weights None: all ones."""
+    where = "rcclAmdExpertCombine"
+    z, zs = _matrix(z, z_stride, rows, hidden, datatype, where, "z")
+    y, ys = _matrix(y, y_stride, tokens, hidden, datatype, where, "y")
+    _check(lib().rcclAmdExpertCombine(z, zs, rows, _whole(weights, tokens * topk, weight_type, where, "weights"), weight_type, y, ys, datatype, tokens, topk, hidden,
+                                      _whole(position, tokens * topk, ncclInt32, where, "position"), _stream(stream)), where)
+
+
+def expert_combine_backward(dy, z, rows, weights, weight_type, dz, dweights, datatype, tokens, topk, hidden, position, offsets=None, counts=None, n_experts=0,
+                            dy_stride=None, z_stride=None, dz_stride=None, stream=None):
+    """rcclAmdExpertCombineBackward: dz[position[t, k]] = weights[t, k] * dy[t], dweights[t, k] = <dy[t], z[position[t, k]]>."""
+    where = "rcclAmdExpertCombineBackward"
+    dy, dys = _matrix(dy, dy_stride, tokens, hidden, datatype, where, "dy")
+    z, zs = _matrix(z, z_stride, rows, hidden, datatype, where, "z")
+    dz, dzs = _matrix(dz, dz_stride, rows, hidden, datatype, where, "dz")
+    _check(lib().rcclAmdExpertCombineBackward(dy, dys, z, zs, rows, _whole(weights, tokens * topk, weight_type, where, "weights"), weight_type, dz, dzs,
+                                              _whole(dweights, tokens * topk, weight_type, where, "dweights"), datatype, tokens, topk, hidden,
+                                              _whole(position, tokens * topk, ncclInt32, where, "position"), _whole(offsets, n_experts + 1, ncclInt32, where, "offsets"),
+                                              _whole(counts, n_experts, ncclInt32, where, "counts"), n_experts, _stream(stream)), where)
 
 
 NO_ALLOC_MAX_BYTES = 256 << 10      # payload limit per rank of rcclAmdAllReduceNoAlloc

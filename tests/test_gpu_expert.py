@@ -1,0 +1,416 @@
+"""Token slots sorted by expert, rows dispatched and combined, and the gradients, against references in 64 bits."""
+import numpy as np
+import pytest
+
+import local_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _types():
+    import torch
+    import rccl_amd as ra
+    return {"f32": (ra.ncclFloat32, torch.float32), "bf16": (ra.ncclBfloat16, torch.bfloat16), "f16": (ra.ncclFloat16, torch.float16)}
+
+
+# ------------------------------------------------------------------ sort
+def _run_sort(ids, first, n, align, wide):
+    import torch
+    import rccl_amd as ra
+    tokens, topk = ids.shape
+    g = 16                                               # guards behind and before every output
+    rows = ra.expert_rows(tokens, topk, n, align)
+    dev = torch.from_numpy(ids.astype(np.int64 if wide else np.int32)).cuda()
+    outs = [torch.full((k + 2 * g,), -77, dtype=torch.int32, device="cuda") for k in (tokens * topk, rows, n + 1, n)]
+    nbytes = ra.expert_sort_bytes(tokens, topk, n)
+    work = torch.full((nbytes + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    cut = [o[g:o.numel() - g] for o in outs]
+    ra.expert_sort(dev, ra.ncclInt64 if wide else ra.ncclInt32, tokens, topk, first, n, align, *cut, workspace=work[:nbytes] if nbytes else None)
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.all(o[:g] == -77) and torch.all(o[o.numel() - g:] == -77)
+    assert torch.all(work[nbytes:] == 0xA5)
+    return [c.cpu().numpy() for c in cut]
+
+
+def _ids(rng, tokens, topk, experts, kind):
+    if kind == "one":                                    # all of them one expert
+        return np.full((tokens, topk), experts - 1, dtype=np.int64)
+    if kind == "padded":
+        ids = rng.integers(0, experts, (tokens, topk))
+        ids[rng.random(tokens) < 0.4] = -1
+        return ids
+    if kind == "skewed":                                 # and duplicates in a token
+        return np.minimum((rng.exponential(0.1, (tokens, topk)) * experts).astype(np.int64), experts - 1)
+    return rng.integers(0, experts, (tokens, topk))
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 2, 63, 64, 65, 127, 513, 1025, 4097, 8193, 70001])
+@pytest.mark.parametrize("topk,experts,first,n,align", [(1, 1, 0, 1, 1), (2, 8, 0, 8, 16), (8, 128, 16, 16, 128), (6, 64, 0, 64, 1), (1, 1000, 0, 1000, 7), (3, 256, 255, 1, 100), (8, 255, 0, 255, 8)])
+def test_sort(tokens, topk, experts, first, n, align):
+    rng = np.random.default_rng(tokens * 31 + n)
+    for i, kind in enumerate(("flat", "padded", "skewed", "one")):
+        if tokens > 5000 and kind in ("flat",):
+            continue
+        ids = _ids(rng, tokens, topk, experts, kind)
+        want = ref.expert_sort(ids, first, n, align)
+        got = _run_sort(ids, first, n, align, wide=bool(i % 2))
+        for name, a, b in zip(("position", "source", "offsets", "counts"), got, want):
+            assert np.array_equal(a, b), (kind, name)
+
+
+@pytest.mark.parametrize("tokens,topk,n", [(5, 64, 1024), (3000, 10, 1024), (1000, 33, 3)])
+def test_sort_at_the_limits(tokens, topk, n):
+    rng = np.random.default_rng(9)
+    ids = _ids(rng, tokens, topk, n, "padded")
+    for a, b in zip(_run_sort(ids, 0, n, 1024, True), ref.expert_sort(ids, 0, n, 1024)):
+        assert np.array_equal(a, b)
+
+
+def test_sort_of_ids_that_are_far_out():
+    """Ids outside every range, the extremes of int64 among them, are dropped."""
+    ids = np.array([[-2 ** 63, 2 ** 63 - 1], [2 ** 32, 2 ** 32 + 5], [5, -1], [6, 4], [7, 5]], dtype=np.int64)
+    for a, b in zip(_run_sort(ids, 5, 2, 4, True), ref.expert_sort(ids, 5, 2, 4)):
+        assert np.array_equal(a, b)
+
+
+def test_sort_without_the_optional_outputs():
+    import torch
+    import rccl_amd as ra
+    ids = np.random.default_rng(3).integers(-1, 8, (50, 2))
+    position = torch.empty(100, dtype=torch.int32, device="cuda")
+    ra.expert_sort(torch.from_numpy(ids).cuda(), ra.ncclInt64, 50, 2, 0, 8, 4, position)
+    assert np.array_equal(position.cpu().numpy(), ref.expert_sort(ids, 0, 8, 4)[0])
+
+
+def test_sort_of_many_slots():
+    """Four million slots of 128 experts: stable, complete and in range (checked by sorting)."""
+    import torch
+    import rccl_amd as ra
+    tokens, topk, n = 500_009, 8, 128
+    ids = torch.randint(-1, n, (tokens, topk), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    position = torch.empty(tokens * topk, dtype=torch.int32, device="cuda")
+    source = torch.empty(ra.expert_rows(tokens, topk, n, 1), dtype=torch.int32, device="cuda")
+    work = torch.empty(ra.expert_sort_bytes(tokens, topk, n), dtype=torch.uint8, device="cuda")
+    ra.expert_sort(ids, ra.ncclInt64, tokens, topk, 0, n, 1, position, source, workspace=work)
+    flat = ids.view(-1)
+    key, order = torch.sort(torch.where(flat < 0, n, flat), stable=True)
+    held = int((key < n).sum())
+    assert torch.equal(source[:held].long(), order[:held]) and torch.all(source[held:] == -1)
+    want = torch.full((tokens * topk,), -1, dtype=torch.int64, device="cuda")
+    want[order[:held]] = torch.arange(held, device="cuda")
+    assert torch.equal(position.long(), want)
+
+
+# ------------------------------------------------------------------ rows
+class Rows:
+    """Routing, and matrices whose rows are `gap` elements further apart than they are long and begin `shift` elements into
+    their storage, with guards on all sides."""
+
+    def __init__(self, tokens, topk, hidden, dtype="bf16", n=8, align=4, gap=0, shift=0, seed=0, experts=None, kind="padded"):
+        self.tokens, self.topk, self.hidden, self.n, self.gap, self.shift = tokens, topk, hidden, n, gap, shift
+        self.rng = np.random.default_rng(seed)
+        self.code, self.torch_type = _types()[dtype]
+        self.dtype = dtype
+        self.ids = _ids(self.rng, tokens, topk, experts or n, kind)
+        self.position, self.source, self.offsets, self.counts = ref.expert_sort(self.ids, 0, n, align)
+        self.rows = self.source.size
+        self.dev = {}
+        import torch
+        for k in ("position", "offsets", "counts"):
+            self.dev[k] = torch.from_numpy(getattr(self, k)).cuda()
+        self.used = np.zeros(self.rows, dtype=bool)
+        self.used[self.position[self.position >= 0]] = True
+        self.pad = np.zeros(self.rows, dtype=bool)
+        for e in range(n):
+            self.pad[self.offsets[e] + self.counts[e]:self.offsets[e + 1]] = True
+
+    def matrix(self, rows, fill=None):
+        """(storage, view of `rows` rows); values of a normal distribution, or `fill`."""
+        import torch
+        wide = self.hidden + self.gap
+        n = (rows + 2) * wide + self.shift + 16
+        if fill is None:
+            flat = torch.from_numpy(self.rng.standard_normal(n).astype(np.float32)).to(self.torch_type).cuda()
+        else:
+            flat = torch.full((n,), fill, dtype=self.torch_type, device="cuda")
+        at = wide + self.shift
+        return flat, flat[at:at + rows * wide].view(rows, wide)[:, :self.hidden] if rows else flat[at:at].view(0, wide)[:, :self.hidden]
+
+    def weights(self, kind):
+        import torch
+        return torch.from_numpy(self.rng.standard_normal((self.tokens, self.topk)).astype(np.float32)).to(_types()[kind][1]).cuda()
+
+    def slots(self):
+        """position as (tokens, topk)."""
+        return self.position.reshape(self.tokens, self.topk)
+
+
+def _outside(flat, view, before):
+    """What of the storage does not belong to the view is as it was."""
+    import torch
+    a, b = flat.clone(), before.clone()
+    for t in (a, b):
+        torch.as_strided(t, view.shape, view.stride(), view.storage_offset()).zero_()
+    return torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def _np64(t):
+    return t.double().cpu().numpy()
+
+
+ROWS = [(1, 1, 1, "bf16", 0, 0), (1, 8, 4096, "bf16", 0, 0), (3, 2, 7, "bf16", 1, 1), (65, 2, 8, "f16", 0, 0), (64, 3, 9, "f32", 3, 1), (130, 8, 63, "f16", 5, 3),
+        (77, 6, 512, "bf16", 8, 0), (50, 64, 130, "bf16", 0, 2), (33, 4, 1000, "f32", 24, 0), (40, 5, 1001, "f32", 0, 0), (300, 2, 2048, "f16", 0, 0),
+        (19, 8, 4097, "bf16", 7, 1), (9, 8, 8200, "f32", 0, 0), (5, 3, 33000, "bf16", 0, 0), (2000, 4, 16, "bf16", 0, 0)]
+
+
+@pytest.mark.parametrize("tokens,topk,hidden,dtype,gap,shift", ROWS)
+def test_dispatch(tokens, topk, hidden, dtype, gap, shift):
+    import torch
+    import rccl_amd as ra
+    r = Rows(tokens, topk, hidden, dtype, gap=gap, shift=shift)
+    _, x = r.matrix(tokens)
+    x[tokens // 2, :] = float("nan")                   # moved like any value
+    for padded in (True, False):
+        flat, out = r.matrix(r.rows, 5.0)
+        before = flat.clone()
+        ra.expert_dispatch(x, out, r.rows, r.code, tokens, topk, hidden, r.dev["position"], **(dict(offsets=r.dev["offsets"], counts=r.dev["counts"], n_experts=r.n) if padded else {}))
+        got, xs = _np64(out), _np64(x)
+        want = np.full((r.rows, hidden), 5.0)
+        for slot, row in enumerate(r.position):
+            if row >= 0:
+                want[row] = xs[slot // topk]
+        if padded:
+            want[r.pad] = 0.0
+        assert np.array_equal(got, want, equal_nan=True)
+        assert _outside(flat, out, before)
+
+
+@pytest.mark.parametrize("tokens,topk,hidden,dtype,gap,shift", ROWS)
+@pytest.mark.parametrize("weights", [None, "f32", "bf16", "f16"])
+def test_combine(tokens, topk, hidden, dtype, gap, shift, weights):
+    import rccl_amd as ra
+    r = Rows(tokens, topk, hidden, dtype, gap=gap, shift=shift, seed=1)
+    _, z = r.matrix(r.rows)
+    z[np.flatnonzero(~r.used)] = float("nan")           # rows without a slot are never part of a sum
+    w = r.weights(weights) if weights else None
+    flat, y = r.matrix(tokens, 5.0)
+    before = flat.clone()
+    ra.expert_combine(z, r.rows, w, _types()[weights][0] if weights else -1, y, r.code, tokens, topk, hidden, r.dev["position"])
+    zs, ws = _np64(z), _np64(w) if weights else np.ones((tokens, topk))
+    want, size = np.zeros((tokens, hidden)), np.zeros((tokens, hidden))
+    for k in range(topk):
+        p = r.slots()[:, k]
+        has = p >= 0
+        want[has] += ws[has, k, None] * zs[p[has]]
+        size[has] += np.abs(ws[has, k, None] * zs[p[has]])
+    # one rounding in each of topk fused multiply-adds of sums that are at most `size`, and half a step of the type at the end
+    bound = 1.01 * topk * ref.U * size
+    bound += (ref.HALF_STEP[dtype] if dtype != "f32" else 0.0) * (np.abs(want) + bound) + ref.TINY[dtype]
+    assert np.all(np.abs(_np64(y) - want) <= bound)
+    assert _outside(flat, y, before)
+
+
+@pytest.mark.parametrize("tokens,topk,hidden,dtype,gap,shift", ROWS)
+@pytest.mark.parametrize("weights", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_combine_backward(tokens, topk, hidden, dtype, gap, shift, weights, in_place):
+    import torch
+    import rccl_amd as ra
+    r = Rows(tokens, topk, hidden, dtype, gap=gap, shift=shift, seed=2)
+    _, dy = r.matrix(tokens)
+    zflat, z = r.matrix(r.rows)
+    z[np.flatnonzero(~r.used)] = float("nan")
+    zs = _np64(z)
+    w = r.weights(weights)
+    dw = torch.full((tokens, topk), 9.0, dtype=w.dtype, device="cuda")
+    flat, dz = (zflat, z) if in_place else r.matrix(r.rows, 5.0)
+    before = flat.clone()
+    ra.expert_combine_backward(dy, z, r.rows, w, _types()[weights][0], dz, dw, r.code, tokens, topk, hidden, r.dev["position"], r.dev["offsets"], r.dev["counts"], r.n)
+    dys, ws = _np64(dy), _np64(w)
+    want = zs.copy() if in_place else np.full((r.rows, hidden), 5.0)
+    want_w, size = np.zeros((tokens, topk)), np.zeros((tokens, topk))
+    for t in range(tokens):
+        for k in range(topk):
+            p = r.slots()[t, k]
+            if p >= 0:
+                want[p] = ws[t, k] * dys[t]
+                want_w[t, k] = np.dot(dys[t], zs[p])
+                size[t, k] = np.dot(np.abs(dys[t]), np.abs(zs[p]))
+    want[r.pad] = 0.0
+    # dz: one rounding in fp32, then half a step of the type.  A row that is behind the last expert is as it was.
+    half = ref.HALF_STEP[dtype] if dtype != "f32" else 0.0
+    bound = (1.01 * ref.U + half * 1.01) * np.abs(want) + ref.TINY[dtype]
+    got = _np64(dz)
+    keep = r.used | r.pad
+    assert np.all(np.abs(got[keep] - want[keep]) <= bound[keep])
+    assert np.array_equal(got[~keep], want[~keep], equal_nan=True)
+    # dw: a lane adds at most 16 products to a sum for each part of the row that a workgroup takes (16384 elements or more,
+    # or the whole row), then 6 + 16 sums join them; the largest row here has 3 parts
+    halfw = ref.HALF_STEP[weights] if weights != "f32" else 0.0
+    bound = 1.01 * (3 * 16 + 3 + 22) * ref.U * size
+    bound += halfw * (np.abs(want_w) + bound) + ref.TINY[weights]
+    assert np.all(np.abs(_np64(dw) - want_w) <= bound)
+    assert _outside(flat, dz, before)
+
+
+def test_gradients_against_differences():
+    """<dy, combine(z, w)> is linear in z and in w: its differences are exact up to rounding, in fp32 with small whole numbers
+    exactly.  The gradient of a dispatch is a combine without weights: <dout, dispatch(x)> = <combine(dout), x>."""
+    import torch
+    import rccl_amd as ra
+    tokens, topk, hidden = 20, 3, 40
+    r = Rows(tokens, topk, hidden, "f32", seed=4)
+    whole = lambda *s: torch.from_numpy(r.rng.integers(-3, 4, s).astype(np.float32)).cuda()  # noqa: E731
+    z, dy, w = whole(r.rows, hidden), whole(tokens, hidden), whole(tokens, topk)
+    dz, dw = torch.zeros_like(z), torch.zeros_like(w)
+    pos = r.dev["position"]
+
+    def loss(z, w):
+        y = torch.empty(tokens, hidden, device="cuda")
+        ra.expert_combine(z, r.rows, w, ra.ncclFloat32, y, ra.ncclFloat32, tokens, topk, hidden, pos)
+        return float((y.double() * dy.double()).sum())
+
+    ra.expert_combine_backward(dy, z, r.rows, w, ra.ncclFloat32, dz, dw, ra.ncclFloat32, tokens, topk, hidden, pos, r.dev["offsets"], r.dev["counts"], r.n)
+    base = loss(z, w)
+    for _ in range(40):
+        i, j = int(r.rng.integers(r.rows)), int(r.rng.integers(hidden))
+        z2 = z.clone()
+        z2[i, j] += 1
+        assert loss(z2, w) - base == (float(dz[i, j]) if r.used[i] else 0.0)
+        t, k = int(r.rng.integers(tokens)), int(r.rng.integers(topk))
+        w2 = w.clone()
+        w2[t, k] += 1
+        assert loss(z, w2) - base == float(dw[t, k])
+    x, dout = whole(tokens, hidden), whole(r.rows, hidden)
+    out, dx = torch.zeros_like(dout), torch.empty_like(x)
+    ra.expert_dispatch(x, out, r.rows, ra.ncclFloat32, tokens, topk, hidden, pos)
+    ra.expert_combine(dout, r.rows, None, -1, dx, ra.ncclFloat32, tokens, topk, hidden, pos)
+    assert float((out.double() * dout.double()).sum()) == float((dx.double() * x.double()).sum())
+
+
+def test_positions_outside_the_rows_are_passed_over():
+    """Positions of a larger order than the buffer has rows (and negative ones): nothing is read or written for them."""
+    import torch
+    import rccl_amd as ra
+    tokens, topk, hidden, rows = 12, 2, 64, 6
+    pos = np.array([0, 6, 5, -1, 2 ** 31 - 1, 1, -2 ** 31, 2, 100, 3, 7, 4] + [-1] * 12, dtype=np.int32)
+    dev = torch.from_numpy(pos).cuda()
+    x = torch.randn(tokens, hidden, device="cuda")
+    flat = torch.full((rows + 20, hidden), 5.0, device="cuda")
+    out = flat[:rows]
+    ra.expert_dispatch(x, out, rows, ra.ncclFloat32, tokens, topk, hidden, dev)
+    assert torch.all(flat[rows:] == 5.0)
+    for slot, p in enumerate(pos):
+        if 0 <= p < rows:
+            assert torch.equal(out[p], x[slot // topk])
+    y = torch.empty(tokens, hidden, device="cuda")
+    ra.expert_combine(out, rows, None, -1, y, ra.ncclFloat32, tokens, topk, hidden, dev)
+    for t in range(tokens):
+        has = [p for p in pos[2 * t:2 * t + 2] if 0 <= p < rows]
+        assert torch.equal(y[t], sum((out[p] for p in has), torch.zeros(hidden, device="cuda")))
+    dz, dw = torch.zeros_like(flat), torch.full((tokens, topk), 9.0, device="cuda")
+    ra.expert_combine_backward(x, out, rows, torch.ones(tokens, topk, device="cuda"), ra.ncclFloat32, dz, dw, ra.ncclFloat32, tokens, topk, hidden, dev)
+    assert not dz[rows:].any()
+    assert torch.equal(dw.view(-1) != 0, torch.from_numpy((pos >= 0) & (pos < rows)).cuda())
+
+
+def test_large_rows_pass_32_bits_of_offset():
+    """A buffer of more than 2^32 bytes: rows at its end."""
+    import torch
+    import rccl_amd as ra
+    hidden, rows = 8192, 300_000                        # 4.9 GB of bf16
+    if torch.cuda.mem_get_info()[0] < 16 * 2 ** 30:
+        pytest.skip("needs 16 GiB of free device memory")
+    tokens = 64
+    pos = torch.arange(rows - tokens, rows, dtype=torch.int32, device="cuda")
+    x = torch.randn(tokens, hidden, device="cuda").to(torch.bfloat16)
+    out = torch.zeros(rows, hidden, dtype=torch.bfloat16, device="cuda")
+    ra.expert_dispatch(x, out, rows, ra.ncclBfloat16, tokens, 1, hidden, pos)
+    assert torch.equal(out[rows - tokens:], x) and not out[:rows - tokens].any()
+    y = torch.empty_like(x)
+    ra.expert_combine(out, rows, None, -1, y, ra.ncclBfloat16, tokens, 1, hidden, pos)
+    assert torch.equal(y, x)
+    w, dw = torch.full((tokens, 1), 2.0, device="cuda"), torch.empty(tokens, 1, device="cuda")
+    ra.expert_combine_backward(x, out, rows, w, ra.ncclFloat32, out, dw, ra.ncclBfloat16, tokens, 1, hidden, pos)
+    assert torch.equal(out[rows - tokens:], 2 * x)
+
+
+def test_no_tokens():
+    import torch
+    import rccl_amd as ra
+    e = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
+    none = torch.empty(0, 2, dtype=torch.int32, device="cuda")
+    out = torch.full((8, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    ra.expert_dispatch(e, out, 8, ra.ncclBfloat16, 0, 2, 64, none)
+    ra.expert_combine(out, 8, None, -1, e, ra.ncclBfloat16, 0, 2, 64, none)
+    w = torch.empty(0, 2, device="cuda")
+    ra.expert_combine_backward(e, out, 8, w, ra.ncclFloat32, torch.empty_like(out), w.clone(), ra.ncclBfloat16, 0, 2, 64, none)
+    assert torch.all(out == 5.0)
+    # tokens, but no rows: everything is dropped
+    y = torch.full((3, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    pos = torch.full((3, 2), -1, dtype=torch.int32, device="cuda")
+    ra.expert_combine(e, 0, None, -1, y, ra.ncclBfloat16, 3, 2, 64, pos)
+    assert not y.any()
+
+
+def test_captured_sort_and_rows_replay():
+    """A layer's sort, dispatch, combine and backward in one graph: each replay with new routing is the eager result."""
+    import torch
+    import rccl_amd as ra
+    tokens, topk, hidden, n, align = 3000, 4, 256, 16, 8
+    rows = ra.expert_rows(tokens, topk, n, align)
+
+    def buffers():
+        i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+        h = lambda r: torch.zeros(r, hidden, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+        return dict(ids=torch.zeros(tokens, topk, dtype=torch.int64, device="cuda"), position=i(tokens, topk), source=i(rows), offsets=i(n + 1), counts=i(n),
+                    work=torch.zeros(max(1, ra.expert_sort_bytes(tokens, topk, n)), dtype=torch.uint8, device="cuda"), x=h(tokens), out=h(rows), y=h(tokens), dz=h(rows),
+                    w=torch.zeros(tokens, topk, device="cuda"), dw=torch.zeros(tokens, topk, device="cuda"))
+
+    def layer(b):
+        ra.expert_sort(b["ids"], ra.ncclInt64, tokens, topk, 0, n, align, b["position"], b["source"], b["offsets"], b["counts"], b["work"])
+        seg = dict(offsets=b["offsets"], counts=b["counts"], n_experts=n)
+        ra.expert_dispatch(b["x"], b["out"], rows, ra.ncclBfloat16, tokens, topk, hidden, b["position"], **seg)
+        ra.expert_combine(b["out"], rows, b["w"], ra.ncclFloat32, b["y"], ra.ncclBfloat16, tokens, topk, hidden, b["position"])
+        ra.expert_combine_backward(b["y"], b["out"], rows, b["w"], ra.ncclFloat32, b["dz"], b["dw"], ra.ncclBfloat16, tokens, topk, hidden, b["position"], **seg)
+
+    a, b = buffers(), buffers()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        layer(b)
+    gen = torch.Generator("cuda").manual_seed(3)
+    for k in range(4):
+        for key, new in (("ids", torch.randint(-1, n + k, (tokens, topk), device="cuda", generator=gen)), ("x", torch.randn(tokens, hidden, device="cuda", generator=gen)),
+                         ("w", torch.rand(tokens, topk, device="cuda", generator=gen))):
+            a[key].copy_(new), b[key].copy_(new)
+        layer(a)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for key in a:
+            assert torch.equal(a[key].view(torch.uint8), b[key].view(torch.uint8)), (k, key)
+
+
+def test_tensor_checks_of_the_python_mirror():
+    import torch
+    import rccl_amd as ra
+    x, out = torch.zeros(4, 64, device="cuda"), torch.zeros(8, 64, device="cuda")
+    pos = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
+    f = ra.ncclFloat32
+    for call in (lambda: ra.expert_dispatch(x.half(), out, 8, f, 4, 2, 64, pos),
+                 lambda: ra.expert_dispatch(x[:3], out, 8, f, 4, 2, 64, pos),
+                 lambda: ra.expert_dispatch(x, out[:, :32], 8, f, 4, 2, 64, pos),
+                 lambda: ra.expert_dispatch(x, out.t(), 8, f, 4, 2, 8, pos),
+                 lambda: ra.expert_dispatch(x, out, 8, f, 4, 2, 64, pos.long()),
+                 lambda: ra.expert_dispatch(x, out, 8, f, 4, 2, 64, pos[:, :1]),
+                 lambda: ra.expert_dispatch(x.cpu(), out, 8, f, 4, 2, 64, pos),
+                 lambda: ra.expert_dispatch(x, x, 4, f, 4, 2, 64, pos),
+                 lambda: ra.expert_dispatch(x, out, 8, f, 4, 2, 64, pos, offsets=torch.zeros(5, dtype=torch.int32, device="cuda"), n_experts=4),
+                 lambda: ra.expert_combine(out, 8, torch.zeros(4, 2, device="cuda"), ra.ncclFloat16, x, f, 4, 2, 64, pos),
+                 lambda: ra.expert_sort(pos, ra.ncclInt32, 4, 2, 0, 4, 1, pos.float()),
+                 lambda: ra.expert_sort(torch.zeros(40000, 1, dtype=torch.int32, device="cuda"), ra.ncclInt32, 40000, 1, 0, 4, 1, torch.zeros(40000, dtype=torch.int32, device="cuda"))):
+        with pytest.raises(ra.NcclError) as e:
+            call()
+        assert e.value.code == ra.ncclInvalidArgument
