@@ -382,32 +382,49 @@ def reduce_copy(dst, srcs, count, datatype, op=ncclSum, stream=None):
 # device, of the element type the call names, and reaching as far as the call will.  Rows may be strided: the stride of a
 # two-dimensional tensor is taken from it.
 
-_TORCH_TYPES = {}
+_TORCH = {}                                     # what the checks need of torch, looked up once: element types by their code
+_current_device = _current_stream = None
 
 
-def _torch_types():
-    if not _TORCH_TYPES:
-        import torch
-        _TORCH_TYPES.update({ncclFloat32: torch.float32, ncclBfloat16: torch.bfloat16, ncclFloat16: torch.float16, ncclFloat64: torch.float64,
-                             ncclInt32: torch.int32, ncclInt64: torch.int64, "current": torch.cuda.current_device})
-    return _TORCH_TYPES
+def _torch():
+    global _current_device, _current_stream
+    import torch
+    torch.cuda.init()
+    _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    _TORCH.update({ncclFloat32: torch.float32, ncclBfloat16: torch.bfloat16, ncclFloat16: torch.float16, ncclFloat64: torch.float64,
+                   ncclInt32: torch.int32, ncclInt64: torch.int64})
 
 
 def _refuse(where, why):
     raise NcclError(ncclInvalidArgument, where, why)
 
 
+def _raw_stream(s):
+    """A hipStream_t as an int; None: torch's current stream."""
+    if s is None:
+        if not _TORCH:
+            _torch()
+        return _current_stream(_current_device())
+    return s if isinstance(s, int) else s.cuda_stream
+
+
+def _unfit(x, datatype, where, name, needed):
+    """Refuses a tensor with what is wrong about it."""
+    if x.get_device() != _current_device():
+        _refuse(where, f"{name} is on {x.device}, not on the current device")
+    if datatype is not None and x.dtype is not _TORCH.get(datatype):
+        _refuse(where, f"{name} is {x.dtype}, the call names type {datatype}")
+    _refuse(where, f"{name} has shape {tuple(x.shape)} and strides {x.stride()}, {needed} needed")
+
+
 def _whole(x, n, datatype, where, name):
     """Address of `n` contiguous elements of `datatype`."""
     if x is None or isinstance(x, int):
         return x
-    t = _torch_types()
-    if not x.is_cuda or x.device.index != t["current"]():
-        _refuse(where, f"{name} is on {x.device}, not on the current device")
-    if x.dtype != t[datatype]:
-        _refuse(where, f"{name} is {x.dtype}, the call names type {datatype}")
-    if x.numel() < n or not x.is_contiguous():
-        _refuse(where, f"{name} has {x.numel()} elements ({'' if x.is_contiguous() else 'not '}contiguous), {n} are needed")
+    if not _TORCH:
+        _torch()
+    if x.get_device() != _current_device() or x.dtype is not _TORCH.get(datatype) or x.numel() < n or not x.is_contiguous():
+        _unfit(x, datatype, where, name, f"{n} contiguous elements are")
     return x.data_ptr()
 
 
@@ -415,41 +432,51 @@ def _matrix(x, stride, rows, hidden, datatype, where, name):
     """(address, stride) of `rows` rows of `hidden` elements of `datatype`, each row contiguous."""
     if x is None or isinstance(x, int):
         return x, hidden if stride is None else stride
-    t = _torch_types()
-    if not x.is_cuda or x.device.index != t["current"]():
-        _refuse(where, f"{name} is on {x.device}, not on the current device")
-    if x.dtype != t[datatype]:
-        _refuse(where, f"{name} is {x.dtype}, the call names type {datatype}")
-    shape = x.shape
-    if len(shape) != 2 or shape[0] < rows or shape[1] < hidden or (shape[1] > 1 and x.stride(1) != 1):
-        _refuse(where, f"{name} has shape {tuple(shape)} and strides {x.stride()}, {rows} contiguous rows of {hidden} are needed")
-    own = x.stride(0) if shape[0] > 1 else max(hidden, x.stride(0))
+    if not _TORCH:
+        _torch()
+    if x.get_device() != _current_device() or x.dtype is not _TORCH.get(datatype):
+        _unfit(x, datatype, where, name, f"{rows} rows of {hidden} contiguous elements are")
+    if x.dim() == 2 and x.size(1) == hidden and x.is_contiguous() and x.numel() >= rows * hidden:
+        own = hidden
+    else:
+        shape = x.shape
+        if len(shape) != 2 or shape[0] < rows or shape[1] < hidden or (shape[1] > 1 and x.stride(1) != 1):
+            _unfit(x, datatype, where, name, f"{rows} rows of {hidden} contiguous elements are")
+        own = x.stride(0)
+        if own < hidden and shape[0] <= 1:      # the stride of a single row says nothing
+            own = hidden
     if stride is not None and stride != own:
         _refuse(where, f"{name} has a row stride of {own}, the call names {stride}")
     return x.data_ptr(), own
 
 
 def _work(x, nbytes, where):
+    """(address, bytes) of a workspace; `nbytes` is what stands behind a bare device pointer."""
     if x is None or isinstance(x, int):
-        return x, nbytes
-    if not x.is_cuda or x.device.index != _torch_types()["current"]():
-        _refuse(where, f"the workspace is on {x.device}, not on the current device")
-    if not x.is_contiguous():
-        _refuse(where, "the workspace is not contiguous")
+        return x, nbytes if x else 0
+    if not _TORCH:
+        _torch()
+    if x.get_device() != _current_device() or not x.is_contiguous():
+        _unfit(x, None, where, "the workspace", "contiguous bytes are")
     return x.data_ptr(), x.numel() * x.element_size()
 
 
 def _host_table(x, columns, where):
     """(address, rows, what keeps it alive) of a C-contiguous host array of 8-byte integers."""
-    import numpy as np
-    a = np.ascontiguousarray(x)
-    if a.dtype.kind not in "iu" or a.dtype.itemsize != 8:
+    face = getattr(x, "__array_interface__", None)
+    if face is not None and face["typestr"] == "<i8" and face["strides"] is None and len(face["shape"]) == (1 if columns is None else 2):
+        a = x
+    else:
+        import numpy as np
+        a = np.ascontiguousarray(x)
         if a.size and a.dtype.kind not in "iu":
             _refuse(where, f"a table of 64-bit integers is needed, got {a.dtype}")
         a = a.astype(np.int64)
-    if a.ndim != (1 if columns is None else 2) or (columns is not None and a.shape[1] != columns):
-        _refuse(where, f"a table of shape {a.shape}")
-    return a.ctypes.data, a.shape[0], a
+        face = a.__array_interface__
+    shape = face["shape"]
+    if len(shape) != (1 if columns is None else 2) or (columns is not None and shape[1] != columns):
+        _refuse(where, f"a table of shape {shape}")
+    return face["data"][0], shape[0], a
 
 
 def adamw_tensor(param, grad, exp_avg, exp_avg_sq, count=None, exp_avg_scale=None, exp_avg_sq_scale=None, copy=None):
@@ -460,11 +487,12 @@ def adamw_tensor(param, grad, exp_avg, exp_avg_sq, count=None, exp_avg_scale=Non
             _refuse("adamw_tensor", "a device pointer needs a count")
         count = param.numel()
     blocks = -(-count // STATE_BLOCK)
+    if tensors and not _TORCH:
+        _torch()
     for x in tensors:
-        if not x.is_cuda or x.device.index != _torch_types()["current"]() or not x.is_contiguous():
-            _refuse("adamw_tensor", f"a tensor on {x.device} with strides {x.stride()}: contiguous ones on the current device are needed")
-        if x.numel() < (blocks if x is exp_avg_scale or x is exp_avg_sq_scale else count):
-            _refuse("adamw_tensor", f"a tensor of {x.numel()} elements for a parameter of {count}")
+        need = blocks if x is exp_avg_scale or x is exp_avg_sq_scale else count
+        if x.get_device() != _current_device() or x.numel() < need or not x.is_contiguous():
+            _unfit(x, None, "adamw_tensor", "a tensor", f"{need} contiguous elements are")
     at = lambda x: 0 if x is None else x if isinstance(x, int) else x.data_ptr()  # noqa: E731
     return [at(param), at(grad), at(exp_avg), at(exp_avg_sq), at(exp_avg_scale), at(exp_avg_sq_scale), at(copy), count]
 
@@ -478,7 +506,7 @@ def adamw(tensors, param_type, grad_type, copy_type=-1, state_type=rcclAmdStateF
     rows, n, keep = _host_table(tensors, 8, where) if len(tensors) else (None, 0, None)
     c = rcclAmdAdamWConfig_t(lr, beta1, beta2, eps, weight_decay, grad_scale, max_norm, step, _whole(step_ptr, 1, ncclInt64, where, "step_ptr"),
                              _whole(lr_ptr, 1, ncclFloat32, where, "lr_ptr"), _whole(sum_sq, 1, ncclFloat64, where, "sum_sq"), seed & 0xFFFFFFFFFFFFFFFF)
-    _check(lib().rcclAmdAdamW(rows, n, param_type, grad_type, copy_type, state_type, ctypes.byref(c), _stream(stream)), where)
+    _check(lib().rcclAmdAdamW(rows, n, param_type, grad_type, copy_type, state_type, ctypes.byref(c), _raw_stream(stream)), where)
     del keep
 
 
@@ -493,15 +521,15 @@ def sum_squares(tensors, counts, datatype, out, workspace, accumulate=False, str
     """rcclAmdSumSquares: out[0] (float64) = sum of the squares of all elements.  `tensors`: a list of torch tensors (counts
     may be None) or an array of device addresses, `counts` an array of their sizes."""
     where = "rcclAmdSumSquares"
-    if len(tensors) and not isinstance(tensors[0], int) and hasattr(tensors[0], "data_ptr"):
+    if isinstance(tensors, (list, tuple)) and tensors and hasattr(tensors[0], "data_ptr"):
         counts = [t.numel() for t in tensors] if counts is None else counts
         tensors = [_whole(t, n, datatype, where, "a tensor") for t, n in zip(tensors, counts)]
     if counts is None or len(counts) != len(tensors):
         _refuse(where, f"{len(tensors)} tensors with other counts")
     ptrs, n, keep = _host_table(tensors, None, where) if len(tensors) else (None, 0, None)
     sizes, _, keep2 = _host_table(counts, None, where) if len(tensors) else (None, 0, None)
-    w, nbytes = _work(workspace, sum_squares_bytes(n), where)
-    _check(lib().rcclAmdSumSquares(ptrs, sizes, n, datatype, _whole(out, 1, ncclFloat64, where, "out"), int(accumulate), w, nbytes, _stream(stream)), where)
+    w, nbytes = _work(workspace, sum_squares_bytes(n) if isinstance(workspace, int) else 0, where)
+    _check(lib().rcclAmdSumSquares(ptrs, sizes, n, datatype, _whole(out, 1, ncclFloat64, where, "out"), int(accumulate), w, nbytes, _raw_stream(stream)), where)
     del keep, keep2
 
 
@@ -522,12 +550,12 @@ def expert_sort(experts, expert_type, tokens, topk, first_expert, n_experts, row
     """rcclAmdExpertSort: rows of the slots in the order of the experts first_expert .. first_expert + n_experts - 1."""
     where = "rcclAmdExpertSort"
     slots = tokens * topk
-    w, nbytes = _work(workspace, 0, where) if workspace is None or not isinstance(workspace, int) else (workspace, expert_sort_bytes(tokens, topk, n_experts))
+    w, nbytes = _work(workspace, expert_sort_bytes(tokens, topk, n_experts) if isinstance(workspace, int) else 0, where)
     _check(lib().rcclAmdExpertSort(_whole(experts, slots, expert_type, where, "experts"), expert_type, tokens, topk, first_expert, n_experts, row_align,
                                    _whole(position, slots, ncclInt32, where, "position"),
                                    _whole(source, expert_rows(tokens, topk, n_experts, row_align), ncclInt32, where, "source"),
                                    _whole(offsets, n_experts + 1, ncclInt32, where, "offsets"), _whole(counts, n_experts, ncclInt32, where, "counts"),
-                                   w, nbytes, _stream(stream)), where)
+                                   w, nbytes, _raw_stream(stream)), where)
 
 
 def expert_dispatch(x, out, rows, datatype, tokens, topk, hidden, position, offsets=None, counts=None, n_experts=0, x_stride=None, out_stride=None, stream=None):
@@ -537,7 +565,7 @@ def expert_dispatch(x, out, rows, datatype, tokens, topk, hidden, position, offs
     out, os_ = _matrix(out, out_stride, rows, hidden, datatype, where, "out")
     _check(lib().rcclAmdExpertDispatch(x, xs, out, os_, rows, datatype, tokens, topk, hidden, _whole(position, tokens * topk, ncclInt32, where, "position"),
                                        _whole(offsets, n_experts + 1, ncclInt32, where, "offsets"), _whole(counts, n_experts, ncclInt32, where, "counts"),
-                                       n_experts, _stream(stream)), where)
+                                       n_experts, _raw_stream(stream)), where)
 
 
 def expert_combine(z, rows, weights, weight_type, y, datatype, tokens, topk, hidden, position, z_stride=None, y_stride=None, stream=None):
@@ -546,7 +574,7 @@ def expert_combine(z, rows, weights, weight_type, y, datatype, tokens, topk, hid
     z, zs = _matrix(z, z_stride, rows, hidden, datatype, where, "z")
     y, ys = _matrix(y, y_stride, tokens, hidden, datatype, where, "y")
     _check(lib().rcclAmdExpertCombine(z, zs, rows, _whole(weights, tokens * topk, weight_type, where, "weights"), weight_type, y, ys, datatype, tokens, topk, hidden,
-                                      _whole(position, tokens * topk, ncclInt32, where, "position"), _stream(stream)), where)
+                                      _whole(position, tokens * topk, ncclInt32, where, "position"), _raw_stream(stream)), where)
 
 
 def expert_combine_backward(dy, z, rows, weights, weight_type, dz, dweights, datatype, tokens, topk, hidden, position, offsets=None, counts=None, n_experts=0,
@@ -559,7 +587,7 @@ def expert_combine_backward(dy, z, rows, weights, weight_type, dz, dweights, dat
     _check(lib().rcclAmdExpertCombineBackward(dy, dys, z, zs, rows, _whole(weights, tokens * topk, weight_type, where, "weights"), weight_type, dz, dzs,
                                               _whole(dweights, tokens * topk, weight_type, where, "dweights"), datatype, tokens, topk, hidden,
                                               _whole(position, tokens * topk, ncclInt32, where, "position"), _whole(offsets, n_experts + 1, ncclInt32, where, "offsets"),
-                                              _whole(counts, n_experts, ncclInt32, where, "counts"), n_experts, _stream(stream)), where)
+                                              _whole(counts, n_experts, ncclInt32, where, "counts"), n_experts, _raw_stream(stream)), where)
 
 
 NO_ALLOC_MAX_BYTES = 256 << 10      # payload limit per rank of rcclAmdAllReduceNoAlloc
