@@ -23,6 +23,7 @@ __global__ __launch_bounds__(RA_SORT_THREADS) void raLocalKernelSortCount(RaSort
   __syncthreads();
   const uint32_t lo = blockIdx.x * tileSlots;                       // (tiles * tileSlots stays below 2^32)
   const uint32_t hi = a.slots - lo < tileSlots ? a.slots : lo + tileSlots;
+#pragma unroll 4
   for (uint32_t i = lo + threadIdx.x; i < hi; i += RA_SORT_THREADS) {
     const int k = keyOf(a, i);
     if (k < a.nExperts) atomicAdd(&hist[k], 1);
@@ -31,28 +32,71 @@ __global__ __launch_bounds__(RA_SORT_THREADS) void raLocalKernelSortCount(RaSort
   for (int e = threadIdx.x; e < a.nExperts; e += RA_SORT_THREADS) a.tileCounts[(size_t)blockIdx.x * a.nExperts + e] = hist[e];
 }
 
+// Where there are many counts: each becomes the sum of those of the tiles before it, and the row behind the last tile the sum
+// of all.  A wave takes one expert, a lane a run of tiles.
+__global__ __launch_bounds__(RA_SORT_THREADS) void raLocalKernelSortScan(RaSortArgs a) {
+  const uint32_t e = blockIdx.x * (RA_SORT_THREADS / 64) + uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (e >= (uint32_t)a.nExperts) return;
+  const uint32_t run = (a.tiles + 63) / 64, lo = lane * run, hi = lo + run < a.tiles ? lo + run : a.tiles;
+  int sum = 0;
+#pragma unroll 8
+  for (uint32_t t = lo; t < hi; t++) sum += a.tileCounts[(size_t)t * a.nExperts + e];
+  int scan = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(scan, d); if (lane >= (uint32_t)d) scan += o; }
+  if (lane == 63) a.tileCounts[(size_t)a.tiles * a.nExperts + e] = scan;
+  scan -= sum;
+#pragma unroll 8
+  for (uint32_t t = lo; t < hi; t++) { const int c = a.tileCounts[(size_t)t * a.nExperts + e]; a.tileCounts[(size_t)t * a.nExperts + e] = scan; scan += c; }
+}
+
+// LDS of the sort: three words for each expert, one for each wave, and for each expert a count of each wave.
+static size_t sortLds(int n) { return (3 * (size_t)n + RA_SORT_THREADS / 64 + 1) * sizeof(int) + (size_t)(RA_SORT_THREADS / 64) * ((n + 1) / 2) * 2 * sizeof(uint16_t); }
+
 template <int ROUNDS>
 __global__ __launch_bounds__(RA_SORT_THREADS) void raLocalKernelSort(RaSortArgs a) {
   constexpr int WAVES = RA_SORT_THREADS / 64;
   extern __shared__ int lds[];
-  const int n = a.nExperts;
-  int* base = lds;                                                  // [n] first row of this tile's slots of an expert
+  const int n = a.nExperts, pitch = (n + 1) / 2 * 2;
+  int* base = lds;                                                  // [n] slots of an expert in earlier tiles, then its first row here
   int* total = lds + n;                                             // [n] slots of an expert in all tiles
-  int* sums = lds + 2 * n;                                          // [WAVES + 1]
-  volatile uint16_t* wc = (volatile uint16_t*)(lds + 2 * n + WAVES + 1);   // [WAVES][n] counts of each wave, at most 64 * ROUNDS
+  int* start = lds + 2 * n;                                         // [n] first row of an expert
+  int* sums = lds + 3 * n;                                          // [WAVES + 1]
+  uint16_t* wc = (uint16_t*)(lds + 3 * n + WAVES + 1);              // [WAVES][pitch] counts of each wave, at most 64 * ROUNDS
   const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6);
-  for (int i = threadIdx.x; i < WAVES * n; i += RA_SORT_THREADS) wc[i] = 0;
-  for (int e = threadIdx.x; e < n; e += RA_SORT_THREADS) { base[e] = 0; total[e] = 0; }
-  __syncthreads();
-
   const uint32_t first = (blockIdx.x * WAVES + wave) * (64u * ROUNDS);
-  const int bits = 32 - __builtin_clz((unsigned)n);                 // keys are 0 .. n
   int key[ROUNDS], rank[ROUNDS];
 #pragma unroll
   for (int r = 0; r < ROUNDS; r++) {
     const uint32_t slot = first + r * 64 + lane;
     key[r] = slot < a.slots ? keyOf(a, slot) : n;
   }
+  for (int i = lane; i < pitch / 2; i += 64) ((int*)(wc + wave * pitch))[i] = 0;     // a wave clears its own
+  for (int e = threadIdx.x; e < n; e += RA_SORT_THREADS) {
+    base[e] = a.scanned ? a.tileCounts[(size_t)blockIdx.x * n + e] : 0;
+    total[e] = a.scanned ? a.tileCounts[(size_t)a.tiles * n + e] : 0;
+  }
+  __syncthreads();
+  // The slots of each expert in all tiles, and in those before this one: groups of threads that hold one expert each take
+  // the tiles in turn.
+  if (a.tiles > 1 && !a.scanned) {
+    const int width = (int)raSortWidth(n);
+    const int e = threadIdx.x & (width - 1);
+    const uint32_t step = RA_SORT_THREADS / width;
+    if (e < n) {
+      int all = 0, before = 0;
+#pragma unroll 8
+      for (uint32_t t = threadIdx.x / width; t < a.tiles; t += step) {
+        const int c = a.tileCounts[(size_t)t * n + e];
+        all += c;
+        before += t < blockIdx.x ? c : 0;
+      }
+      if (all) atomicAdd(&total[e], all);
+      if (before) atomicAdd(&base[e], before);
+    }
+  }
+  const int bits = 32 - __builtin_clz((unsigned)n);                 // keys are 0 .. n
+  volatile uint16_t* mine = wc + wave * pitch;                      // LDS operations of one wave are done in order
 #pragma unroll
   for (int r = 0; r < ROUNDS; r++) {
     uint64_t peers = ~0ull;
@@ -64,26 +108,21 @@ __global__ __launch_bounds__(RA_SORT_THREADS) void raLocalKernelSort(RaSortArgs 
     const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(peers >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)peers, 0));
     int before = 0;
     if (key[r] < n) {
-      before = wc[wave * n + key[r]];                               // LDS operations of one wave are done in order
-      if (below == 0) wc[wave * n + key[r]] = (uint16_t)(before + __popcll(peers));
+      before = mine[key[r]];
+      if (below == 0) mine[key[r]] = (uint16_t)(before + __popcll(peers));
     }
     rank[r] = before + below;
   }
-  if (a.tiles > 1)
-    for (uint32_t i = threadIdx.x; i < a.tiles * (uint32_t)n; i += RA_SORT_THREADS) {
-      const int c = a.tileCounts[i];
-      if (c) {
-        atomicAdd(&total[i % n], c);
-        if (i / n < blockIdx.x) atomicAdd(&base[i % n], c);
-      }
-    }
   __syncthreads();
-  // Thread e: the expert's counts of the waves before each wave; its slots in all tiles.
+  // Thread e: the expert's counts of the waves before each wave, its rows.
   int padded = 0;
   const int e = threadIdx.x;
   if (e < n) {
-    int run = 0;
-    for (int w = 0; w < WAVES; w++) { const int c = wc[w * n + e]; wc[w * n + e] = (uint16_t)run; run += c; }
+    int c[WAVES], run = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) c[w] = wc[w * pitch + e];
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) { wc[w * pitch + e] = (uint16_t)run; run += c[w]; }
     if (a.tiles == 1) total[e] = run;
     padded = (total[e] + a.rowAlign - 1) / a.rowAlign * a.rowAlign;
   }
@@ -92,22 +131,18 @@ __global__ __launch_bounds__(RA_SORT_THREADS) void raLocalKernelSort(RaSortArgs 
   for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(scan, d); if (lane >= d) scan += o; }
   if (lane == 63) sums[wave] = scan;
   __syncthreads();
-  if (threadIdx.x == 0) { int run = 0; for (int w = 0; w < WAVES; w++) { const int c = sums[w]; sums[w] = run; run += c; } sums[WAVES] = run; }
-  __syncthreads();
-  const int start = sums[wave] + scan - padded;                     // first row of expert e
+  int earlier = 0, used = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) { const int c = sums[w]; earlier += w < wave ? c : 0; used += c; }
   if (e < n) {
-    base[e] += start;
+    const int from = earlier + scan - padded;
+    base[e] += from;
+    start[e] = from;
     if (blockIdx.x == 0) {
-      if (a.offsets) { a.offsets[e] = start; if (e == n - 1) a.offsets[n] = start + padded; }
+      if (a.offsets) { a.offsets[e] = from; if (e == n - 1) a.offsets[n] = from + padded; }
       if (a.counts) a.counts[e] = total[e];
     }
-    // Rows without a slot: the padding of each expert by one workgroup, what is behind the last expert by all of them.
-    if (a.source && e % a.tiles == blockIdx.x)
-      for (int row = start + total[e]; row < start + padded; row++) a.source[row] = -1;
   }
-  if (a.source)
-    for (uint32_t row = (uint32_t)sums[WAVES] + blockIdx.x * RA_SORT_THREADS + threadIdx.x; row < a.rows; row += a.tiles * RA_SORT_THREADS)
-      a.source[row] = -1;
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < ROUNDS; r++) {
@@ -115,22 +150,29 @@ __global__ __launch_bounds__(RA_SORT_THREADS) void raLocalKernelSort(RaSortArgs 
     if (slot >= a.slots) continue;
     int row = -1;
     if (key[r] < n) {
-      row = base[key[r]] + wc[wave * n + key[r]] + rank[r];
+      row = base[key[r]] + wc[wave * pitch + key[r]] + rank[r];
       if (a.source) a.source[row] = (int32_t)slot;
     }
     a.position[slot] = row;
   }
+  if (!a.source) return;
+  // Rows without a slot: the padding of an expert by a wave of one workgroup, what is behind the last expert by all of them.
+  for (uint32_t x = blockIdx.x + wave * a.tiles; x < (uint32_t)n; x += WAVES * a.tiles) {
+    const int from = start[x] + total[x], to = x + 1 < (uint32_t)n ? start[x + 1] : used;
+    for (int row = from + lane; row < to; row += 64) a.source[row] = -1;
+  }
+  for (uint32_t row = (uint32_t)used + blockIdx.x * RA_SORT_THREADS + threadIdx.x; row < a.rows; row += a.tiles * RA_SORT_THREADS) a.source[row] = -1;
 }
 
 hipError_t raLaunchSort(const RaSortArgs& a, hipStream_t s) {
   const uint32_t rounds = raSortRounds(a.slots);
-  const int waves = RA_SORT_THREADS / 64;
   if (a.tiles > 1) hipLaunchKernelGGL(raLocalKernelSortCount, dim3(a.tiles), dim3(RA_SORT_THREADS), a.nExperts * sizeof(int), s, a, RA_SORT_THREADS * rounds);
-  const size_t lds = (2 * (size_t)a.nExperts + waves + 1) * sizeof(int) + (size_t)waves * a.nExperts * sizeof(uint16_t);
+  if (a.scanned) hipLaunchKernelGGL(raLocalKernelSortScan, dim3((a.nExperts + 15) / 16), dim3(RA_SORT_THREADS), 0, s, a);
   switch (rounds) {
-    case 1: hipLaunchKernelGGL((raLocalKernelSort<1>), dim3(a.tiles), dim3(RA_SORT_THREADS), lds, s, a); break;
-    case 4: hipLaunchKernelGGL((raLocalKernelSort<4>), dim3(a.tiles), dim3(RA_SORT_THREADS), lds, s, a); break;
-    default: hipLaunchKernelGGL((raLocalKernelSort<8>), dim3(a.tiles), dim3(RA_SORT_THREADS), lds, s, a); break;
+    case 1: hipLaunchKernelGGL((raLocalKernelSort<1>), dim3(a.tiles), dim3(RA_SORT_THREADS), sortLds(a.nExperts), s, a); break;
+    case 2: hipLaunchKernelGGL((raLocalKernelSort<2>), dim3(a.tiles), dim3(RA_SORT_THREADS), sortLds(a.nExperts), s, a); break;
+    case 4: hipLaunchKernelGGL((raLocalKernelSort<4>), dim3(a.tiles), dim3(RA_SORT_THREADS), sortLds(a.nExperts), s, a); break;
+    default: hipLaunchKernelGGL((raLocalKernelSort<8>), dim3(a.tiles), dim3(RA_SORT_THREADS), sortLds(a.nExperts), s, a); break;
   }
   return hipGetLastError();
 }
@@ -154,23 +196,32 @@ template <typename T> static __device__ __forceinline__ u32x4 fromFloats(typenam
   typedef T vec __attribute__((ext_vector_type(Pack<T>::N)));
   return __builtin_bit_cast(u32x4, __builtin_convertvector(f, vec));
 }
-// The pack at element `at` of a row of `hidden` elements; past its end there are zeros, and nothing is written.
-template <typename T> static __device__ __forceinline__ u32x4 loadPack(const T* row, size_t at, size_t hidden) {
+// A pack of a row.  STREAM: the access does not ask for a place in the caches.
+template <bool STREAM, typename T> static __device__ __forceinline__ u32x4 wholePack(const T* p) {
+  return STREAM ? __builtin_nontemporal_load((const u32x4_u2*)p) : *(const u32x4_u2*)p;
+}
+template <bool STREAM, typename T> static __device__ __forceinline__ void storeWhole(T* p, u32x4 x) {
+  if (STREAM) __builtin_nontemporal_store(x, (u32x4_u2*)p);
+  else *(u32x4_u2*)p = x;
+}
+// The pack at element `at` of a row of `hidden` elements, where the row may end inside it: there are zeros past its end, and
+// nothing is written there.
+template <bool STREAM, typename T> static __device__ __forceinline__ u32x4 loadPack(const T* row, size_t at, size_t hidden) {
   constexpr int N = Pack<T>::N;
-  if (at + N <= hidden) return *(const u32x4_u2*)(row + at);
+  if (at + N <= hidden) return wholePack<STREAM>(row + at);
   typedef T vec __attribute__((ext_vector_type(N)));
   vec v = {};
 #pragma unroll
-  for (int i = 0; i < N; i++) if (at + i < hidden) v[i] = row[at + i];
+  for (int i = 0; i < N - 1; i++) if (at + i < hidden) v[i] = row[at + i];
   return __builtin_bit_cast(u32x4, v);
 }
-template <typename T> static __device__ __forceinline__ void storePack(T* row, size_t at, size_t hidden, u32x4 p) {
+template <bool STREAM, typename T> static __device__ __forceinline__ void storePack(T* row, size_t at, size_t hidden, u32x4 p) {
   constexpr int N = Pack<T>::N;
-  if (at + N <= hidden) { *(u32x4_u2*)(row + at) = p; return; }
+  if (at + N <= hidden) { storeWhole<STREAM>(row + at, p); return; }
   typedef T vec __attribute__((ext_vector_type(N)));
   const vec v = __builtin_bit_cast(vec, p);
 #pragma unroll
-  for (int i = 0; i < N; i++) if (at + i < hidden) row[at + i] = v[i];
+  for (int i = 0; i < N - 1; i++) if (at + i < hidden) row[at + i] = v[i];
 }
 static __device__ __forceinline__ float weightOf(const void* w, int type, size_t i) {
   if (type == ncclFloat32) return ((const float*)w)[i];
@@ -181,7 +232,7 @@ static __device__ __forceinline__ float weightOf(const void* w, int type, size_t
 static __device__ __forceinline__ int laneInt(int x, int k) { return __builtin_amdgcn_readlane(x, k); }
 static __device__ __forceinline__ float laneFloat(float x, int k) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), k)); }
 
-// The padding rows of the segments are set to zero by the workgroups behind those of the tokens, RA_PAD_GROUPS for each expert.
+// The padding rows of the segments are set to zero by the workgroups behind those of the slots, RA_PAD_GROUPS for each expert.
 #define RA_PAD_GROUPS 4
 template <typename T> static __device__ __forceinline__ void padRows(const RaRowsArgs& a, uint32_t group) {
   const int e = (int)(group / RA_PAD_GROUPS);
@@ -191,50 +242,49 @@ template <typename T> static __device__ __forceinline__ void padRows(const RaRow
   if (row < 0) return;
   for (; row < end; row += RA_PAD_GROUPS * waves)
     for (size_t at = (threadIdx.x & 63) * Pack<T>::N; at < a.hidden; at += 64 * Pack<T>::N)
-      storePack((T*)a.out + (size_t)row * a.outStride, at, a.hidden, u32x4{0, 0, 0, 0});
+      storePack<false>((T*)a.out + (size_t)row * a.outStride, at, a.hidden, u32x4{0, 0, 0, 0});
 }
 
-// Dispatch.  A wave takes 64 * U packs of one token's row, reads them once and writes them to each of the token's slots.
-#define RA_ROWS_THREADS 256
-template <typename T, int U>
-__global__ __launch_bounds__(RA_ROWS_THREADS) void raLocalKernelDispatch(RaRowsArgs a, uint32_t groups, uint32_t parts) {
+// Dispatch.  A wave takes one slot's row (or a part of it, where there are too few slots to fill the GPU), 8 packs in flight
+// for each lane: long runs of one row are what the time follows here.  16384 tokens of 8 slots, 4096 bf16 elements (1.24 GB
+// to move): 8 KiB in one go 0.220 ms, 4 KiB 0.225, 2 KiB 0.235; a wave that reads a row once and writes all of the token's
+// rows 0.236; streaming accesses 0.225 to 0.250.  The waves of a token's slots are in one workgroup, so that its row comes
+// from HBM once.  Sixteen waves of a compute unit at a time (RA_FEW_WAVES): with 20, 24 and 32 the runs of more rows mix, and
+// the time is 0.226, 0.239 and 0.244 ms.
+#define RA_SLOT_THREADS 1024         // at most; see slotThreads
+#define RA_FEW_WAVES __attribute__((amdgpu_waves_per_eu(4, 4)))
+template <typename T>
+__global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES void raLocalKernelDispatch(RaRowsArgs a, uint32_t groups, uint32_t parts, size_t partElems) {
+  constexpr int N = Pack<T>::N, U = 8;
   if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
-  const int lane = threadIdx.x & 63;
-  const uint64_t unit = (uint64_t)blockIdx.x * (RA_ROWS_THREADS / 64) + uniform(threadIdx.x >> 6);
-  const size_t token = unit / parts;
-  if (token >= a.tokens) return;
-  const int32_t pos = lane < a.topk ? a.position[token * a.topk + lane] : -1;
-  uint64_t slots = __ballot(pos >= 0 && (size_t)pos < a.rows);
-  if (!slots) return;
-  const T* x = (const T*)a.in + token * a.inStride;
-  const size_t at = ((size_t)(unit % parts) * 64 * U + lane) * Pack<T>::N;
-  u32x4 p[U];
+  const uint64_t unit = (uint64_t)blockIdx.x * (blockDim.x >> 6) + uniform(threadIdx.x >> 6);
+  const size_t slot = unit / parts;
+  if (slot >= a.tokens * a.topk) return;
+  const int32_t pos = a.position[slot];
+  if (pos < 0 || (size_t)pos >= a.rows) return;
+  const T* x = (const T*)a.in + slot / a.topk * a.inStride;
+  T* out = (T*)a.out + (size_t)pos * a.outStride;
+  const size_t begin = unit % parts * partElems, end = begin + partElems < a.hidden ? begin + partElems : a.hidden;
+  size_t at = begin + (threadIdx.x & 63) * N;
+  for (; at + (U - 1) * 64 * N + N <= end; at += U * 64 * N) {
+    u32x4 p[U];
 #pragma unroll
-  for (int u = 0; u < U; u++) p[u] = loadPack(x, at + u * 64 * Pack<T>::N, a.hidden);
-  for (; slots; slots &= slots - 1) {
-    T* row = (T*)a.out + (size_t)laneInt(pos, __builtin_ctzll(slots)) * a.outStride;
+    for (int u = 0; u < U; u++) p[u] = wholePack<false>(x + at + u * 64 * N);
 #pragma unroll
-    for (int u = 0; u < U; u++) storePack(row, at + u * 64 * Pack<T>::N, a.hidden, p[u]);
+    for (int u = 0; u < U; u++) storeWhole<false>(out + at + u * 64 * N, p[u]);
   }
+  for (; at < end; at += 64 * N) storePack<false>(out, at, end, loadPack<false>(x, at, end));
 }
 
-// Combine.  A wave takes 64 * U packs of one token's row and adds those of its slots in the order of k, four rows in flight.
-template <typename T, int U>
-__global__ __launch_bounds__(RA_ROWS_THREADS) void raLocalKernelCombine(RaRowsArgs a, uint32_t parts) {
+// Combine.  A wave takes 64 * U packs of one token's row and adds those of its slots in the order of k, F rows in flight; the
+// part in which a row ends, and all of it where there are few tokens, in runs of 64 packs.  The same micro-batch back (1.21 GB):
+// U = 4 and F = 4 0.205 ms, U = 2 0.209, U = 4 and F = 2 0.206 (F = 8 0.202, but with more registers than eight waves of a
+// compute unit's SIMD have), accesses that are not streaming 0.235.
+#define RA_COMBINE_THREADS 256
+template <typename T, int U, bool WHOLE>
+static __device__ __forceinline__ void combineAt(const RaRowsArgs& a, size_t token, size_t at, uint64_t slots, int32_t pos, float w) {
   constexpr int N = Pack<T>::N, F = 4;
   typedef typename Pack<T>::floats floats;
-  const int lane = threadIdx.x & 63;
-  const uint64_t unit = (uint64_t)blockIdx.x * (RA_ROWS_THREADS / 64) + uniform(threadIdx.x >> 6);
-  const size_t token = unit / parts;
-  if (token >= a.tokens) return;
-  int32_t pos = -1;
-  float w = 1.f;
-  if (lane < a.topk) {
-    pos = a.position[token * a.topk + lane];
-    if (a.weightType >= 0) w = weightOf(a.weights, a.weightType, token * a.topk + lane);
-  }
-  uint64_t slots = __ballot(pos >= 0 && (size_t)pos < a.rows);
-  const size_t at = ((size_t)(unit % parts) * 64 * U + lane) * N;
   floats sum[U];
 #pragma unroll
   for (int u = 0; u < U; u++) sum[u] = floats{};
@@ -251,7 +301,7 @@ __global__ __launch_bounds__(RA_ROWS_THREADS) void raLocalKernelCombine(RaRowsAr
       wk[f] = laneFloat(w, k);
       const T* z = (const T*)a.in + (size_t)laneInt(pos, k) * a.inStride;
 #pragma unroll
-      for (int u = 0; u < U; u++) p[f][u] = loadPack(z, at + u * 64 * N, a.hidden);
+      for (int u = 0; u < U; u++) p[f][u] = WHOLE ? wholePack<true>(z + at + u * 64 * N) : loadPack<true>(z, at + u * 64 * N, a.hidden);
     }
 #pragma unroll
     for (int f = 0; f < F; f++) {
@@ -266,90 +316,125 @@ __global__ __launch_bounds__(RA_ROWS_THREADS) void raLocalKernelCombine(RaRowsAr
   }
   T* y = (T*)a.out + token * a.outStride;
 #pragma unroll
-  for (int u = 0; u < U; u++) storePack(y, at + u * 64 * N, a.hidden, fromFloats<T>(sum[u]));
+  for (int u = 0; u < U; u++) {
+    if (WHOLE) storeWhole<true>(y + at + u * 64 * N, fromFloats<T>(sum[u]));
+    else storePack<true>(y, at + u * 64 * N, a.hidden, fromFloats<T>(sum[u]));
+  }
 }
-
-// The gradients of combine.  A workgroup takes one token: its row of dy stays in registers (a part of the row at a time,
-// where it is longer than the workgroup holds) while the rows of its slots pass; each wave adds its part of a slot's
-// product into its own word in LDS.
 template <typename T>
-__global__ __launch_bounds__(1024) void raLocalKernelCombineBackward(RaRowsArgs a, uint32_t groups) {
-  constexpr int N = Pack<T>::N, U = 2;
-  typedef typename Pack<T>::floats floats;
-  __shared__ float dots[16][RA_ROWS_MAX_TOPK];
-  if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
-  const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6), waves = (int)(blockDim.x >> 6);
-  const size_t token = blockIdx.x;
+__global__ __launch_bounds__(RA_COMBINE_THREADS) void raLocalKernelCombine(RaRowsArgs a, uint32_t parts, size_t partElems) {
+  constexpr int N = Pack<T>::N, U = 4;
+  const int lane = threadIdx.x & 63;
+  const uint64_t unit = (uint64_t)blockIdx.x * (RA_COMBINE_THREADS / 64) + uniform(threadIdx.x >> 6);
+  const size_t token = unit / parts;
+  if (token >= a.tokens) return;
   int32_t pos = -1;
-  float w = 0.f;
+  float w = 1.f;
   if (lane < a.topk) {
     pos = a.position[token * a.topk + lane];
-    w = weightOf(a.weights, a.weightType, token * a.topk + lane);
-    dots[wave][lane] = 0.f;
+    if (a.weightType >= 0) w = weightOf(a.weights, a.weightType, token * a.topk + lane);
   }
-  const uint64_t all = __ballot(pos >= 0 && (size_t)pos < a.rows);
-  const T* dy = (const T*)a.in + token * a.inStride;
-  if (all)
-    for (size_t part = 0; part < a.hidden; part += (size_t)waves * 64 * U * N) {
-      const size_t at = part + ((size_t)wave * 64 * U + lane) * N;
-      floats d[U];
+  const uint64_t slots = __ballot(pos >= 0 && (size_t)pos < a.rows);
+  size_t at = unit % parts * partElems;
+  const size_t end = at + partElems < a.hidden ? at + partElems : a.hidden;
+  for (; at + U * 64 * N <= end; at += U * 64 * N) combineAt<T, U, true>(a, token, at + lane * N, slots, pos, w);
+  for (; at < end; at += 64 * N) combineAt<T, 1, false>(a, token, at + lane * N, slots, pos, w);
+}
+
+// The sum of x over the wave, in lane 63: inside rows of 16 lanes, then rows 0 and 2 into 1 and 3, then 1 into 3 (DPP moves).
+template <int CTRL, int ROWS> static __device__ __forceinline__ float dppAdd(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWS, 0xF, false));
+}
+static __device__ __forceinline__ float waveSum63(float x) {
+  x = dppAdd<0xB1, 0xF>(x);
+  x = dppAdd<0x4E, 0xF>(x);
+  x = dppAdd<0x141, 0xF>(x);
+  x = dppAdd<0x140, 0xF>(x);
+  x = dppAdd<0x142, 0xA>(x);
+  return dppAdd<0x143, 0xC>(x);
+}
+
+// w * dy of a pack; the pack's part of <dy, z> is added to `dot`.
+template <typename T> static __device__ __forceinline__ u32x4 gradients(u32x4 z, u32x4 dy, float w, float& dot) {
+  const typename Pack<T>::floats zf = toFloats<T>(z), d = toFloats<T>(dy);
+  typename Pack<T>::floats g;
 #pragma unroll
-      for (int u = 0; u < U; u++) d[u] = toFloats<T>(loadPack(dy, at + u * 64 * N, a.hidden));
-      for (uint64_t slots = all; slots; slots &= slots - 1) {
-        const int k = __builtin_ctzll(slots);
-        const size_t row = (size_t)laneInt(pos, k);
-        const float wk = laneFloat(w, k);
-        const T* z = (const T*)a.z + row * a.zStride;
-        T* dz = (T*)a.out + row * a.outStride;
-        float dot = 0.f;
+  for (int i = 0; i < Pack<T>::N; i++) { dot = __builtin_fmaf(d[i], zf[i], dot); g[i] = w * d[i]; }
+  return fromFloats<T>(g);
+}
+
+// The gradients of combine.  A wave takes one slot: dz's row is written while z's row passes, and their product stays in the
+// wave.  Runs of 8 KiB as in dispatch: half of the slots of 16384 tokens (1.23 GB) 0.232 ms, runs of 4 KiB 0.240, 2 KiB 0.243; a
+// workgroup for each token, its row in registers, 0.234 at best.
+template <typename T>
+__global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES void raLocalKernelCombineBackward(RaRowsArgs a, uint32_t groups) {
+  constexpr int N = Pack<T>::N, U = 8;
+  if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
+  const size_t slot = (size_t)blockIdx.x * (blockDim.x >> 6) + uniform(threadIdx.x >> 6);
+  if (slot >= a.tokens * a.topk) return;
+  const int32_t pos = a.position[slot];
+  float dot = 0.f;
+  if (pos >= 0 && (size_t)pos < a.rows) {
+    const float w = weightOf(a.weights, a.weightType, slot);
+    const T* dy = (const T*)a.in + slot / a.topk * a.inStride;
+    const T* z = (const T*)a.z + (size_t)pos * a.zStride;
+    T* dz = (T*)a.out + (size_t)pos * a.outStride;
+    size_t at = (threadIdx.x & 63) * N;
+    for (; at + (U - 1) * 64 * N + N <= a.hidden; at += U * 64 * N) {
+      u32x4 p[U], q[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          const floats zf = toFloats<T>(loadPack(z, at + u * 64 * N, a.hidden));
-          floats g;
+      for (int u = 0; u < U; u++) { p[u] = wholePack<true>(z + at + u * 64 * N); q[u] = wholePack<false>(dy + at + u * 64 * N); }
 #pragma unroll
-          for (int i = 0; i < N; i++) { dot = __builtin_fmaf(d[u][i], zf[i], dot); g[i] = wk * d[u][i]; }
-          storePack(dz, at + u * 64 * N, a.hidden, fromFloats<T>(g));
-        }
-#pragma unroll
-        for (int s = 32; s > 0; s >>= 1) dot += __shfl_xor(dot, s);
-        if (lane == 0) dots[wave][k] += dot;
+      for (int u = 0; u < U; u++) {
+        storeWhole<true>(dz + at + u * 64 * N, gradients<T>(p[u], q[u], w, dot));
+        __builtin_amdgcn_sched_barrier(0);                 // one pack as floats at a time: the packs take half of the registers
       }
     }
-  __syncthreads();
-  if (wave == 0 && lane < a.topk) {
-    float sum = 0.f;
-    for (int v = 0; v < waves; v++) sum += dots[v][lane];
-    const size_t slot = token * a.topk + lane;
-    if (a.weightType == ncclFloat32) ((float*)a.dweights)[slot] = sum;
-    else if (a.weightType == ncclBfloat16) ((__bf16*)a.dweights)[slot] = (__bf16)sum;
-    else ((_Float16*)a.dweights)[slot] = (_Float16)sum;
+    for (; at < a.hidden; at += 64 * N)
+      storePack<true>(dz, at, a.hidden, gradients<T>(loadPack<true>(z, at, a.hidden), loadPack<false>(dy, at, a.hidden), w, dot));
+    dot = waveSum63(dot);
+  }
+  if ((threadIdx.x & 63) == 63) {
+    if (a.weightType == ncclFloat32) ((float*)a.dweights)[slot] = dot;
+    else if (a.weightType == ncclBfloat16) ((__bf16*)a.dweights)[slot] = (__bf16)dot;
+    else ((_Float16*)a.dweights)[slot] = (_Float16)dot;
   }
 }
 
 static uint32_t padGroups(const RaRowsArgs& a) { return a.offsets ? (uint32_t)a.nExperts * RA_PAD_GROUPS : 0; }
 
+// Threads of a workgroup of slots: whole tokens, eight waves or nearly so.
+static int slotThreads(int topk) { return 64 * (topk <= 8 ? 8 / topk * topk : topk <= 16 ? topk : 8); }
+static uint64_t groupsOf(uint64_t units, int threads) { return (units + threads / 64 - 1) / (threads / 64); }
+
 template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_t s) {
-  constexpr int U = 2;
-  const uint64_t parts = (a.hidden + 64 * U * Pack<T>::N - 1) / (64 * U * Pack<T>::N);
-  const uint64_t groups = (a.tokens * parts + RA_ROWS_THREADS / 64 - 1) / (RA_ROWS_THREADS / 64);
+  const uint64_t slots = (uint64_t)a.tokens * a.topk, step = 64 * Pack<T>::N;
+  // parts of a row, down to 64 packs, where there are fewer than 4096 waves otherwise
+  uint64_t parts = 1, most = (a.hidden + step - 1) / step;
+  while (parts < most && slots * parts < 4096) parts *= 2;
+  const size_t partElems = ((a.hidden + parts - 1) / parts + step - 1) / step * step;
+  parts = (a.hidden + partElems - 1) / partElems;
+  const int threads = slotThreads(a.topk);
+  const uint64_t groups = groupsOf(slots * parts, threads);
   if (groups + padGroups(a) > 0x7FFFFFFF) return hipErrorInvalidValue;
   if (groups + padGroups(a) == 0) return hipSuccess;
-  hipLaunchKernelGGL((raLocalKernelDispatch<T, U>), dim3((uint32_t)groups + padGroups(a)), dim3(RA_ROWS_THREADS), 0, s, a, (uint32_t)groups, (uint32_t)parts);
+  hipLaunchKernelGGL(raLocalKernelDispatch<T>, dim3((uint32_t)groups + padGroups(a)), dim3(threads), 0, s, a, (uint32_t)groups, (uint32_t)parts, partElems);
   return hipGetLastError();
 }
 template <typename T> static hipError_t combine(const RaRowsArgs& a, hipStream_t s) {
-  constexpr int U = 2;
-  const uint64_t parts = (a.hidden + 64 * U * Pack<T>::N - 1) / (64 * U * Pack<T>::N);
-  const uint64_t groups = (a.tokens * parts + RA_ROWS_THREADS / 64 - 1) / (RA_ROWS_THREADS / 64);
+  const uint64_t step = 64 * Pack<T>::N;
+  // four runs of 64 packs for each wave, or one where that leaves fewer than 4096 waves
+  const size_t partElems = a.tokens * ((a.hidden + 4 * step - 1) / (4 * step)) < 4096 ? step : 4 * step;
+  const uint64_t parts = (a.hidden + partElems - 1) / partElems, groups = groupsOf(a.tokens * parts, RA_COMBINE_THREADS);
   if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((raLocalKernelCombine<T, U>), dim3((uint32_t)groups), dim3(RA_ROWS_THREADS), 0, s, a, (uint32_t)parts);
+  hipLaunchKernelGGL(raLocalKernelCombine<T>, dim3((uint32_t)groups), dim3(RA_COMBINE_THREADS), 0, s, a, (uint32_t)parts, partElems);
   return hipGetLastError();
 }
 template <typename T> static hipError_t combineBackward(const RaRowsArgs& a, hipStream_t s) {
-  const size_t packs = (a.hidden + Pack<T>::N - 1) / Pack<T>::N;
-  const size_t waves = packs <= 128 ? 1 : packs >= 16 * 128 ? 16 : (packs + 127) / 128;
-  if (a.tokens + padGroups(a) > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((raLocalKernelCombineBackward<T>), dim3((uint32_t)a.tokens + padGroups(a)), dim3((uint32_t)waves * 64), 0, s, a, (uint32_t)a.tokens);
+  const int threads = slotThreads(a.topk);
+  const uint64_t groups = groupsOf((uint64_t)a.tokens * a.topk, threads);
+  if (groups + padGroups(a) > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((raLocalKernelCombineBackward<T>), dim3((uint32_t)groups + padGroups(a)), dim3(threads), 0, s, a, (uint32_t)groups);
   return hipGetLastError();
 }
 #define RA_BY_TYPE(fn)                                    \

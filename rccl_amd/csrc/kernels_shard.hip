@@ -26,16 +26,18 @@ template <typename T> static __device__ __forceinline__ void store4(T* p, f32x4 
   typedef T vec __attribute__((ext_vector_type(4)));
   __builtin_nontemporal_store(__builtin_convertvector(x, vec), (typename Vec<T>::four*)p);
 }
-// `left` elements from p on exist (0 .. 4 of them are this lane's).
+// The same where only `left` (1 .. 3) of the four elements exist; the others are zeros.
 template <typename T> static __device__ __forceinline__ f32x4 load4(const T* p, int left) {
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 4; i++) if (i < left) x[i] = (float)p[i];
+  x[0] = (float)p[0];
+  if (left > 1) x[1] = (float)p[1];
+  if (left > 2) x[2] = (float)p[2];
   return x;
 }
 template <typename T> static __device__ __forceinline__ void store4(T* p, f32x4 x, int left) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) if (i < left) p[i] = (T)x[i];
+  p[0] = (T)x[0];
+  if (left > 1) p[1] = (T)x[1];
+  if (left > 2) p[2] = (T)x[2];
 }
 
 // 32 bits that depend on all of x: two rounds of xor-shift and multiplication by an odd constant (2^32 over the golden
@@ -48,13 +50,16 @@ static __device__ __forceinline__ uint32_t mix(uint32_t x) {
 static __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 static __device__ __forceinline__ float uniform(float x) { return __uint_as_float(uniform(__float_as_uint(x))); }
 
-// Which of the launch's tensors chunk b belongs to: the number of tensors that begin at or before it, less one.
-static __device__ __forceinline__ uint32_t findTensor(const uint32_t* first, uint32_t n, uint32_t b) {
-  uint32_t t = 0;
-  for (uint32_t k = 0; k < n; k += 64) {
-    const uint32_t i = k + (threadIdx.x & 63);
-    t += (uint32_t)__popcll(__ballot(i < n && first[i < n ? i : 0] <= b));
-  }
+// Which of the launch's tensors chunk b belongs to: the number of tensors that begin at or before it, less one.  All loads
+// are on their way before the first is waited for.
+template <int MAX> static __device__ __forceinline__ uint32_t findTensor(const uint32_t* first, uint32_t n, uint32_t b) {
+  if (n == 1) return 0;
+  uint32_t f[(MAX + 63) / 64], t = 0;
+  const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 0; k < (MAX + 63) / 64; k++) f[k] = k * 64 + lane < n ? first[k * 64 + lane] : ~0u;
+#pragma unroll
+  for (int k = 0; k < (MAX + 63) / 64; k++) t += (uint32_t)__popcll(__ballot(f[k] <= b));
   return uniform(t - 1);
 }
 
@@ -121,30 +126,42 @@ template <typename P, typename G, bool MX> struct Row {
   f32x4 p, g, fm, fv;
   uint32_t qm, qv, xm, xv;
 
-  template <bool FULL> __device__ __forceinline__ void load(size_t at, int left) {
-    if (FULL) { p = load4(param + at); g = load4(grad + at); }
-    else { p = load4(param + at, left); g = load4(grad + at, left); }
-    if constexpr (MX) {
-      if (FULL) { qm = __builtin_nontemporal_load((const u32_u*)(cm + at)); qv = __builtin_nontemporal_load((const u32_u*)(cv + at)); }
-      else {
-        qm = qv = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) if (i < left) { qm |= (uint32_t)cm[at + i] << (8 * i); qv |= (uint32_t)cv[at + i] << (8 * i); }
+  // A lane's elements of a row are at .. at + 3; `left` of them exist (4 in every lane where WHOLE).
+  template <bool WHOLE> __device__ __forceinline__ void load(size_t at, int left) {
+    if (WHOLE || left >= 4) {
+      p = load4(param + at); g = load4(grad + at);
+      if constexpr (MX) { qm = __builtin_nontemporal_load((const u32_u*)(cm + at)); qv = __builtin_nontemporal_load((const u32_u*)(cv + at)); }
+      else { fm = load4(m + at); fv = load4(v + at); }
+    } else {
+      p = g = fm = fv = f32x4{0.f, 0.f, 0.f, 0.f};
+      qm = qv = 0;
+      if (left > 0) {
+        p = load4(param + at, left); g = load4(grad + at, left);
+        if constexpr (MX) {
+          qm = cm[at]; qv = cv[at];
+          if (left > 1) { qm |= (uint32_t)cm[at + 1] << 8; qv |= (uint32_t)cv[at + 1] << 8; }
+          if (left > 2) { qm |= (uint32_t)cm[at + 2] << 16; qv |= (uint32_t)cv[at + 2] << 16; }
+        } else { fm = load4(m + at, left); fv = load4(v + at, left); }
       }
+    }
+    if constexpr (MX) {
       xm = xv = 0;
-      if (FULL || left > 0) { xm = sm[at / RCCL_AMD_STATE_BLOCK]; xv = sv[at / RCCL_AMD_STATE_BLOCK]; }
-    } else if (FULL) { fm = load4(m + at); fv = load4(v + at); }
-    else { fm = load4(m + at, left); fv = load4(v + at, left); }
+      if (WHOLE || left > 0) { xm = sm[at / RCCL_AMD_STATE_BLOCK]; xv = sv[at / RCCL_AMD_STATE_BLOCK]; }
+    }
   }
-  template <bool FULL> __device__ __forceinline__ void storeCopy(size_t at, int left) {
+  template <typename C> __device__ __forceinline__ void storeAs(C* to, bool whole, int left) {
+    if (whole) store4(to, p);
+    else if (left > 0) store4(to, p, left);
+  }
+  __device__ __forceinline__ void storeCopy(size_t at, bool whole, int left) {
     if (copyType < 0) return;
-    if (copyType == ncclFloat32) { if (FULL) store4((float*)copy + at, p); else store4((float*)copy + at, p, left); }
-    else if (copyType == ncclBfloat16) { if (FULL) store4((__bf16*)copy + at, p); else store4((__bf16*)copy + at, p, left); }
-    else { if (FULL) store4((_Float16*)copy + at, p); else store4((_Float16*)copy + at, p, left); }
+    if (copyType == ncclFloat32) storeAs((float*)copy + at, whole, left);
+    else if (copyType == ncclBfloat16) storeAs((__bf16*)copy + at, whole, left);
+    else storeAs((_Float16*)copy + at, whole, left);
   }
   // Division and square root are the correctly rounded ones; nothing is contracted, so that a rounding of an 8-bit state
   // does not depend on how this is compiled.
-  template <bool FULL> __device__ __forceinline__ void update(const Scalars& s, size_t at, int left, uint32_t key) {
+  template <bool WHOLE> __device__ __forceinline__ void update(const Scalars& s, size_t at, int left, uint32_t key) {
     f32x4 r;
     if constexpr (MX) { fm = decode4(qm, xm); r = decode4(qv, xv); fv = r * r; }
 #pragma unroll
@@ -155,13 +172,11 @@ template <typename P, typename G, bool MX> struct Row {
       r[i] = __builtin_sqrtf(fv[i]);
       p[i] = p[i] * s.decay - s.stepSize * (fm[i] / (r[i] * s.rootC2 + s.eps));
     }
-    if (FULL) store4(param + at, p); else store4(param + at, p, left);
-    storeCopy<FULL>(at, left);
+    const bool whole = WHOLE || left >= 4;
+    storeAs(param + at, whole, left);
+    storeCopy(at, whole, left);
     if constexpr (MX) {
-      if (!FULL) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) if (i >= left) { fm[i] = 0.f; r[i] = 0.f; }
-      }
+      // (what does not exist is zero: its gradient and its moments were)
       const uint32_t em = scaleOf(maxOf8(bitsMax(fm))), ev = scaleOf(maxOf8(bitsMax(r)));
       uint32_t rm[4], rv[4];
 #pragma unroll
@@ -171,25 +186,43 @@ template <typename P, typename G, bool MX> struct Row {
         rv[i] = (h >> 16) << 4 | 8u;
       }
       const uint32_t nm = encode4<false>(fm, em, rm), nv = encode4<true>(r, ev, rv);
-      if (FULL) { __builtin_nontemporal_store(nm, (u32_u*)(cm + at)); __builtin_nontemporal_store(nv, (u32_u*)(cv + at)); }
-      else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) if (i < left) { cm[at + i] = (uint8_t)(nm >> (8 * i)); cv[at + i] = (uint8_t)(nv >> (8 * i)); }
+      if (whole) { __builtin_nontemporal_store(nm, (u32_u*)(cm + at)); __builtin_nontemporal_store(nv, (u32_u*)(cv + at)); }
+      else if (left > 0) {
+        cm[at] = (uint8_t)nm; cv[at] = (uint8_t)nv;
+        if (left > 1) { cm[at + 1] = (uint8_t)(nm >> 8); cv[at + 1] = (uint8_t)(nv >> 8); }
+        if (left > 2) { cm[at + 2] = (uint8_t)(nm >> 16); cv[at + 2] = (uint8_t)(nv >> 16); }
       }
-      if ((threadIdx.x & 7) == 0 && (FULL || left > 0)) { sm[at / RCCL_AMD_STATE_BLOCK] = (uint8_t)em; sv[at / RCCL_AMD_STATE_BLOCK] = (uint8_t)ev; }
-    } else if (FULL) { store4(m + at, fm); store4(v + at, fv); }
-    else { store4(m + at, fm, left); store4(v + at, fv, left); }
+      if ((threadIdx.x & 7) == 0 && (WHOLE || left > 0)) { sm[at / RCCL_AMD_STATE_BLOCK] = (uint8_t)em; sv[at / RCCL_AMD_STATE_BLOCK] = (uint8_t)ev; }
+    } else if (whole) { store4(m + at, fm); store4(v + at, fv); }
+    else if (left > 0) { store4(m + at, fm, left); store4(v + at, fv, left); }
   }
 };
 
 template <typename P, typename G, bool MX>
-__global__ __launch_bounds__(RA_ADAMW_THREADS) void raLocalKernelAdamW(RaAdamWArgs a) {
-  constexpr int U = 2;                                      // rows in flight for each wave
+__global__ __launch_bounds__(RA_ADAMW_THREADS) __attribute__((amdgpu_waves_per_eu(1, MX ? 8 : 4))) void raLocalKernelAdamW(RaAdamWArgs a) {
+  // Rows in flight for each wave.  fp32 states: one, and one row for each wave in all, so that the workgroups that run at a
+  // time stream through one window of memory: a shard of 67 million elements (1.88 GB) 0.310 ms = 6.07 TB/s, and with 2, 4 and 16
+  // rows for each wave 0.313, 0.320 and 0.350; accesses that are not streaming 0.369.  8-bit states have 100 VALU cycles for
+  // each element, as long as memory takes, and a longer start: two rows at a time of four, 0.177 ms (1.08 GB, 6.1 TB/s).
+  // Of fp32 states no more than 16 waves run on a compute unit, which is 1.5 % faster than 32: fewer runs of memory at a time.
+  constexpr int U = MX ? 2 : 1;
   constexpr uint32_t STEP = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW;
-  const uint32_t t = findTensor(a.first, a.n, blockIdx.x);
-  const uint64_t* w = a.words + (size_t)t * a.stride;
-  const size_t count = w[RA_W_COUNT];
-  const size_t begin = (size_t)(blockIdx.x - a.first[t]) * a.chunk;
+  uint32_t t, chunk0;
+  size_t count, offset = 0;
+  const uint64_t* w;
+  if (a.stride) {
+    t = findTensor<RA_ADAMW_MAX>(a.general.first, a.n, blockIdx.x);
+    chunk0 = a.general.first[t];
+    w = a.general.words + (size_t)t * a.stride;
+    count = w[RA_W_COUNT];
+  } else {
+    t = findTensor<RA_ADAMW_FLAT>(a.flat.first, a.n, blockIdx.x);
+    chunk0 = a.flat.first[t];
+    w = a.flat.base;
+    count = a.flat.count[t];
+    offset = a.flat.offset[t];
+  }
+  const size_t begin = (size_t)(blockIdx.x - chunk0) * a.chunk;
   const size_t end = begin + a.chunk < count ? begin + a.chunk : count;
 
   Scalars s = {a.b1, a.omb1, a.b2, a.omb2, a.eps, a.decay, a.stepSize, a.rootC2, a.coef};
@@ -212,24 +245,17 @@ __global__ __launch_bounds__(RA_ADAMW_THREADS) void raLocalKernelAdamW(RaAdamWAr
   Row<P, G, MX> row[U];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    row[u].param = (P*)w[RA_W_PARAM]; row[u].grad = (const G*)w[RA_W_GRAD];
-    if constexpr (MX) { row[u].cm = (uint8_t*)w[RA_W_M]; row[u].cv = (uint8_t*)w[RA_W_V]; row[u].sm = (uint8_t*)w[RA_W_MS]; row[u].sv = (uint8_t*)w[RA_W_VS]; }
-    else { row[u].m = (float*)w[RA_W_M]; row[u].v = (float*)w[RA_W_V]; }
+    row[u].param = (P*)w[RA_W_PARAM] + offset; row[u].grad = (const G*)w[RA_W_GRAD] + offset;
+    if constexpr (MX) {
+      row[u].cm = (uint8_t*)w[RA_W_M] + offset; row[u].cv = (uint8_t*)w[RA_W_V] + offset;
+      row[u].sm = (uint8_t*)w[RA_W_MS] + offset / RCCL_AMD_STATE_BLOCK; row[u].sv = (uint8_t*)w[RA_W_VS] + offset / RCCL_AMD_STATE_BLOCK;
+    } else { row[u].m = (float*)w[RA_W_M] + offset; row[u].v = (float*)w[RA_W_V] + offset; }
     row[u].copy = a.copyWord >= 0 ? (void*)w[a.copyWord] : nullptr;
     row[u].copyType = row[u].copy ? a.copyType : -1;
+    if (row[u].copy) row[u].copy = (char*)row[u].copy + offset * (a.copyType == ncclFloat32 ? 4 : 2);
   }
   const uint32_t lane4 = (threadIdx.x & 63) * 4;
   size_t r = begin + uniform(threadIdx.x >> 6) * RA_ADAMW_ROW;
-  if (!go) {                                                // a skipped step: only the copies are written
-    if (row[0].copyType >= 0)
-      for (; r < end; r += STEP) {
-        const size_t at = r + lane4;
-        const int left = at < end ? (end - at < 4 ? (int)(end - at) : 4) : 0;
-        row[0].p = load4(row[0].param + at, left);
-        row[0].template storeCopy<false>(at, left);
-      }
-    return;
-  }
   uint32_t key = 0;
   if constexpr (MX) {
     key = mix((uint32_t)a.seed + 0x9E3779B9u);
@@ -237,26 +263,27 @@ __global__ __launch_bounds__(RA_ADAMW_THREADS) void raLocalKernelAdamW(RaAdamWAr
     key = mix(key + (uint32_t)step);
     key = uniform(mix(a.ordinal + t + key));
   }
-  for (; r + (U - 1) * STEP + RA_ADAMW_ROW <= end; r += U * STEP) {
+  // (the high word of an element's index belongs to its random bits too)
+  if (U > 1 && go)
+    for (; r + (U - 1) * STEP + RA_ADAMW_ROW <= end; r += U * STEP) {
 #pragma unroll
-    for (int u = 0; u < U; u++) row[u].template load<true>(r + u * STEP + lane4, 4);
+      for (int u = 0; u < U; u++) row[u].template load<true>(r + u * STEP + lane4, 4);
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const size_t at = r + u * STEP;
-      const uint32_t k = at >> 32 ? mix(key ^ (uint32_t)(at >> 32)) : key;
-      row[u].template update<true>(s, at + lane4, 4, k);
+      for (int u = 0; u < U; u++) {
+        const size_t at = r + u * STEP;
+        row[u].template update<true>(s, at + lane4, 4, at >> 32 ? mix(key ^ (uint32_t)(at >> 32)) : key);
+      }
     }
-  }
   for (; r < end; r += STEP) {
     const size_t at = r + lane4;
-    const uint32_t k = r >> 32 ? mix(key ^ (uint32_t)(r >> 32)) : key;
-    if (r + RA_ADAMW_ROW <= end) {
-      row[0].template load<true>(at, 4);
-      row[0].template update<true>(s, at, 4, k);
-    } else {
-      const int left = at < end ? (end - at < 4 ? (int)(end - at) : 4) : 0;
+    const int left = at < end ? (end - at < 4 ? (int)(end - at) : 4) : 0;
+    if (go) {
       row[0].template load<false>(at, left);
-      row[0].template update<false>(s, at, left, k);
+      row[0].template update<false>(s, at, left, r >> 32 ? mix(key ^ (uint32_t)(r >> 32)) : key);
+    } else if (row[0].copyType >= 0) {                      // a skipped step: only the copies are written
+      if (left >= 4) row[0].p = load4(row[0].param + at);
+      else if (left > 0) row[0].p = load4(row[0].param + at, left);
+      row[0].storeCopy(at, left >= 4, left);
     }
   }
 }
@@ -308,7 +335,7 @@ template <typename T> static __device__ __forceinline__ f32x4 load4Cached(const 
 }
 template <typename T>
 __global__ __launch_bounds__(RA_SUMSQ_THREADS) void raLocalKernelSumSq(RaSumSqArgs a) {
-  const uint32_t t = findTensor(a.first, a.n, blockIdx.x);
+  const uint32_t t = findTensor<RA_SUMSQ_MAX>(a.first, a.n, blockIdx.x);
   const T* x = (const T*)a.ptr[t];
   const uint32_t count = a.count[t];
   const uint64_t begin = (uint64_t)(blockIdx.x - a.first[t]) * a.chunk;
@@ -327,7 +354,7 @@ __global__ __launch_bounds__(RA_SUMSQ_THREADS) void raLocalKernelSumSq(RaSumSqAr
       for (int i = 0; i < 4; i++) sum[i] = __builtin_fma((double)v[u][i], (double)v[u][i], sum[i]);
   }
   for (; r < end; r += STEP) {
-    const f32x4 v = load4(x + r, end - r < 4 ? (int)(end - r) : 4);
+    const f32x4 v = end - r < 4 ? load4(x + r, (int)(end - r)) : load4Cached(x + r);
 #pragma unroll
     for (int i = 0; i < 4; i++) sum[i] = __builtin_fma((double)v[i], (double)v[i], sum[i]);
   }

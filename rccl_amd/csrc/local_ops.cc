@@ -22,13 +22,43 @@
 
 static bool isFloat(int t) { return t == ncclFloat32 || t == ncclBfloat16 || t == ncclFloat16; }
 static bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
-static const uint64_t kMaxElements = 1ull << 43;      // of one call: byte offsets and chunk numbers stay far from overflow
+static const uint64_t kMaxElements = 1ull << 40;      // of one call: byte offsets and chunk numbers stay far from overflow
+static const size_t kMaxRow = 1u << 28;               // elements of a row and its stride: so do the offsets of 2^31 rows
 
 // x^n by squaring, in the same steps as the kernel that reads the step number from the device.
 static double powN(double x, int64_t n) {
   double r = 1.0;
   for (; n > 0; n >>= 1, x *= x) if (n & 1) r *= x;
   return r;
+}
+
+// The words of a tensor: its count and the pointers that its form of the call uses.
+static void describe(const rcclAmdAdamWTensor_t& t, bool mx, bool copies, uint64_t* w) {
+  w[RA_W_COUNT] = t.count;
+  w[RA_W_PARAM] = (uint64_t)t.param; w[RA_W_GRAD] = (uint64_t)t.grad; w[RA_W_M] = (uint64_t)t.expAvg; w[RA_W_V] = (uint64_t)t.expAvgSq;
+  if (mx) { w[RA_W_MS] = (uint64_t)t.expAvgScale; w[RA_W_VS] = (uint64_t)t.expAvgSqScale; }
+  if (copies) w[mx ? RA_W_VS + 1 : RA_W_V + 1] = (uint64_t)t.copy;
+}
+
+// Whether every tensor is the same run of elements of its flat buffers, counted from the tensor with the lowest address,
+// whose pointers go to `base`: param + o, grad + o, the moments + o (their scales + o / 32) and the copy + o, or no copies.
+static bool liesFlat(const rcclAmdAdamWTensor_t* tensors, int n, bool mx, size_t ps, size_t gs, size_t cs, uint64_t* base) {
+  const rcclAmdAdamWTensor_t* b = nullptr;
+  for (int i = 0; i < n; i++) if (tensors[i].count && (!b || tensors[i].param < b->param)) b = &tensors[i];
+  if (!b) return false;
+  const size_t ss = mx ? 1 : 4;
+  for (int i = 0; i < n; i++) {
+    const rcclAmdAdamWTensor_t& t = tensors[i];
+    if (t.count == 0) continue;
+    const uintptr_t bytes = (uintptr_t)t.param - (uintptr_t)b->param, o = bytes / ps;
+    if (bytes % ps || o > 0xFFFFFFFF || t.count > 0xFFFFFFFF) return false;
+    if ((uintptr_t)t.grad - (uintptr_t)b->grad != o * gs || (uintptr_t)t.expAvg - (uintptr_t)b->expAvg != o * ss || (uintptr_t)t.expAvgSq - (uintptr_t)b->expAvgSq != o * ss) return false;
+    if (mx && (o % RCCL_AMD_STATE_BLOCK || (uintptr_t)t.expAvgScale - (uintptr_t)b->expAvgScale != o / RCCL_AMD_STATE_BLOCK ||
+               (uintptr_t)t.expAvgSqScale - (uintptr_t)b->expAvgSqScale != o / RCCL_AMD_STATE_BLOCK)) return false;
+    if (!t.copy != !b->copy || (t.copy && (uintptr_t)t.copy - (uintptr_t)b->copy != o * cs)) return false;
+  }
+  describe(*b, mx, b->copy != nullptr, base);
+  return true;
 }
 
 RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntensors, ncclDataType_t paramType, ncclDataType_t gradType,
@@ -68,30 +98,35 @@ RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntenso
   a.rootC2 = (float)(1.0 / sqrt(1.0 - powN(c.beta2, c.step)));
   a.coef = (float)c.gradScale;
   a.copyType = copies ? (int)copyType : -1;
-  a.copyWord = copies ? (mx ? 7 : 5) : -1;
-  a.stride = (mx ? 7 : 5) + (copies ? 1 : 0);
-  const int fit = RA_ADAMW_WORDS / (int)a.stride < RA_ADAMW_MAX ? RA_ADAMW_WORDS / (int)a.stride : RA_ADAMW_MAX;
-  // A chunk is the work of one workgroup: four rows (1024 elements) where there is little, so that small tensors spread
-  // over the GPU, up to sixteen times that for long ones, where a workgroup's start would show.
+  a.copyWord = copies ? (mx ? RA_W_VS + 1 : RA_W_V + 1) : -1;
+  a.stride = (mx ? RA_W_VS : RA_W_V) + (copies ? 2 : 1);
+  const uint32_t stride = a.stride;
+  const int general = RA_ADAMW_WORDS / (int)stride < RA_ADAMW_MAX ? RA_ADAMW_WORDS / (int)stride : RA_ADAMW_MAX;
+  const bool flat = ntensors > general && liesFlat(tensors, ntensors, mx, ps, gs, cs, a.flat.base);
+  const int fit = flat ? RA_ADAMW_FLAT : general;
+  if (flat) a.stride = 0;
+  // A chunk is the work of one workgroup: four rows (1024 elements), or up to four times that for 8-bit states where there
+  // is much to do (see the kernel).
   const uint64_t unit = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW;
   for (int lo = 0; lo < ntensors; lo += fit) {
     const int n = ntensors - lo < fit ? ntensors - lo : fit;
     uint64_t elements = 0, chunks = 0;
     for (int i = 0; i < n; i++) elements += tensors[lo + i].count;
     if (elements == 0) continue;
-    uint64_t chunk = (elements / 4096 + unit - 1) / unit * unit;
-    chunk = chunk < unit ? unit : chunk > 16 * unit ? 16 * unit : chunk;
+    uint64_t chunk = mx ? (elements / 4096 + unit - 1) / unit * unit : unit;
+    chunk = chunk < unit ? unit : chunk > 4 * unit ? 4 * unit : chunk;
     for (int i = 0; i < n; i++) {
       const rcclAmdAdamWTensor_t& t = tensors[lo + i];
-      uint64_t* w = a.words + (size_t)i * a.stride;
-      w[RA_W_COUNT] = t.count;
-      w[RA_W_PARAM] = (uint64_t)t.param; w[RA_W_GRAD] = (uint64_t)t.grad; w[RA_W_M] = (uint64_t)t.expAvg; w[RA_W_V] = (uint64_t)t.expAvgSq;
-      if (mx) { w[RA_W_MS] = (uint64_t)t.expAvgScale; w[RA_W_VS] = (uint64_t)t.expAvgSqScale; }
-      if (copies) w[a.copyWord] = (uint64_t)t.copy;
-      a.first[i] = (uint32_t)chunks;
+      if (flat) {
+        a.flat.offset[i] = t.count ? (uint32_t)(((uintptr_t)t.param - a.flat.base[RA_W_PARAM]) / ps) : 0;
+        a.flat.count[i] = (uint32_t)t.count;
+        a.flat.first[i] = (uint32_t)chunks;
+      } else {
+        describe(t, mx, copies, a.general.words + (size_t)i * stride);
+        a.general.first[i] = (uint32_t)chunks;
+      }
       chunks += (t.count + chunk - 1) / chunk;
     }
-    if (chunks > 0x7FFFFFFF) RA_REFUSE("%s: too many elements", fn);
     a.n = (uint32_t)n; a.chunk = (uint32_t)chunk; a.ordinal = (uint32_t)lo;
     RA_LAUNCH(fn, raLaunchAdamW(a, paramType, gradType, mx, (uint32_t)chunks, stream));
   }
@@ -167,7 +202,7 @@ RA_API ncclResult_t rcclAmdExpertSortBytes(size_t tokens, int topk, int nExperts
   RA_CHECK(checkSlots(fn, tokens, topk));
   if (nExperts < 1 || nExperts > RA_SORT_MAX_EXPERTS || !workspaceBytes) RA_REFUSE("%s: %d experts, 1 .. %d supported, or a null argument", fn, nExperts, RA_SORT_MAX_EXPERTS);
   const uint64_t tiles = raSortTiles((uint64_t)tokens * topk);
-  *workspaceBytes = tiles > 1 ? (size_t)tiles * nExperts * sizeof(int32_t) : 0;
+  *workspaceBytes = tiles > 1 ? (size_t)(tiles + 1) * nExperts * sizeof(int32_t) : 0;
   return ncclSuccess;
 }
 
@@ -191,6 +226,7 @@ RA_API ncclResult_t rcclAmdExpertSort(const void* experts, ncclDataType_t expert
   a.tileCounts = (int32_t*)workspace; a.slots = (uint32_t)slots; a.rows = (uint32_t)rows;
   a.tiles = slots ? (uint32_t)raSortTiles(slots) : 1;
   a.nExperts = nExperts; a.rowAlign = rowAlign; a.idBytes = (int)raTypeSize(expertType);
+  a.scanned = raSortScanned(a.tiles, nExperts);
   RA_LAUNCH(fn, raLaunchSort(a, stream));
   return ncclSuccess;
 }
@@ -200,10 +236,10 @@ static ncclResult_t checkRows(const char* fn, const RaRowsArgs& a, int datatype,
   RA_CHECK(checkSlots(fn, a.tokens, a.topk));
   if (!isFloat(datatype)) RA_REFUSE("%s: type %d is not float32, bfloat16 or float16", fn, datatype);
   const size_t s = raTypeSize(datatype);
-  if (a.hidden < 1 || a.hidden > 0x7FFFFFFF) RA_REFUSE("%s: rows of %zu elements", fn, a.hidden);
+  if (a.hidden < 1 || a.hidden > kMaxRow) RA_REFUSE("%s: rows of %zu elements", fn, a.hidden);
   if (a.rows > 0x7FFFFFFF) RA_REFUSE("%s: %zu rows, 2^31 - 1 at most", fn, a.rows);
   if (a.inStride < a.hidden || a.outStride < a.hidden || (a.z && a.zStride < a.hidden)) RA_REFUSE("%s: a stride is below the %zu elements of a row", fn, a.hidden);
-  if (a.inStride > kMaxElements / 4096 || a.outStride > kMaxElements / 4096 || a.zStride > kMaxElements / 4096) RA_REFUSE("%s: a stride is too large", fn);
+  if (a.inStride > kMaxRow || a.outStride > kMaxRow || a.zStride > kMaxRow) RA_REFUSE("%s: a stride is too large", fn);
   if (!a.offsets != !a.counts) RA_REFUSE("%s: offsets and counts belong together", fn);
   if (a.offsets && (a.nExperts < 1 || a.nExperts > RA_SORT_MAX_EXPERTS)) RA_REFUSE("%s: %d experts, 1 .. %d supported", fn, a.nExperts, RA_SORT_MAX_EXPERTS);
   if (a.weightType >= 0 && !isFloat(a.weightType)) RA_REFUSE("%s: weight type %d is not float32, bfloat16 or float16", fn, a.weightType);

@@ -8,17 +8,26 @@
 
 // ------------------------------------------------------------------ AdamW, sum of squares
 // Everything a launch needs travels in its arguments (at most 4 KiB): no table in device memory, nothing to allocate or to
-// keep alive, and a captured launch stays valid.  A tensor takes `stride` words: the pointers the launch uses (a form
-// without copies or scales leaves theirs out, so that more tensors fit) and its element count.
-#define RA_ADAMW_WORDS 420           // 8-byte words of tensor descriptions: 84 tensors of 5 words, 52 of 8
-#define RA_ADAMW_MAX 84
+// keep alive, and a captured launch stays valid.  In the general form a tensor takes `stride` words: the pointers the launch
+// uses (a form without copies or scales leaves theirs out, so that more tensors fit) and its element count.  Tensors that
+// lie alike in flat buffers, as shards do, need only their element offset and count: 300 fit into a launch.
+#define RA_ADAMW_WORDS 414           // 8-byte words of tensor descriptions: 82 tensors of 5 words, 51 of 8
+#define RA_ADAMW_MAX 82
+#define RA_ADAMW_FLAT 300
 #define RA_ADAMW_THREADS 256
 #define RA_ADAMW_ROW 256             // elements a wave takes in one step: 4 for each lane
 enum { RA_W_COUNT = 0, RA_W_PARAM = 1, RA_W_GRAD = 2, RA_W_M = 3, RA_W_V = 4, RA_W_MS = 5, RA_W_VS = 6 };   // then copy
 
-struct RaAdamWArgs {
+struct RaAdamWGeneral {
   uint64_t words[RA_ADAMW_WORDS];
   uint32_t first[RA_ADAMW_MAX];      // first chunk (= workgroup) of each tensor
+};
+struct RaAdamWFlat {
+  uint64_t base[8];                  // the pointers of the tensor at offset 0, in the places of a general tensor's words
+  uint32_t offset[RA_ADAMW_FLAT], count[RA_ADAMW_FLAT], first[RA_ADAMW_FLAT];
+};
+struct RaAdamWArgs {
+  union { RaAdamWGeneral general; RaAdamWFlat flat; };
   double lr, beta1, beta2, weightDecay, gradScale, maxNorm;
   const int64_t* stepPtr;
   const float* lrPtr;
@@ -26,7 +35,7 @@ struct RaAdamWArgs {
   int64_t step;
   uint64_t seed;
   float b1, omb1, b2, omb2, eps, decay, stepSize, rootC2, coef;   // the same in fp32, where nothing is read from the device
-  uint32_t n, stride, chunk;         // tensors, words for each, elements of a chunk (a multiple of 4 rows)
+  uint32_t n, stride, chunk;         // tensors, words for each (0: flat), elements of a chunk (a multiple of 4 rows)
   uint32_t ordinal;                  // place of the first tensor in the call
   int copyWord, copyType;            // word of the copy's pointer (-1: none), its ncclDataType_t
 };
@@ -58,16 +67,27 @@ struct RaSortArgs {
   int32_t* source;
   int32_t* offsets;
   int32_t* counts;
-  int32_t* tileCounts;               // [tiles][nExperts], tiles > 1
+  int32_t* tileCounts;               // [tiles + 1][nExperts], tiles > 1
   uint32_t slots, rows, tiles;
   int nExperts, rowAlign, idBytes;
+  bool scanned;                      // raSortScanned
 };
-// Rounds of 64 slots a wave takes in one tile, by the number of slots (a tile is RA_SORT_THREADS * rounds).
-static inline uint32_t raSortRounds(uint64_t slots) { return slots <= 1024 ? 1 : slots <= 4096 ? 4 : 8; }
+// Rounds of 64 slots a wave takes in one tile (a tile is RA_SORT_THREADS * rounds): one tile up to 4096 slots, which is one
+// launch; beyond that tiles that grow with the number of slots, as every tile adds up or scans the counts of all.  In us, with
+// 2, 4 and 8 rounds: 131072 slots of 256 experts 12.6, 13.2, 17.2; 524288 of 384 experts 20.7, 19.1, 22.8; 4.2 million of 128 experts
+// 107, 71, 58.
+static inline uint32_t raSortRounds(uint64_t slots) {
+  return slots <= 1024 ? 1 : slots <= 2048 ? 2 : slots <= 4096 ? 4 : slots <= 1u << 18 ? 2 : slots <= 1u << 21 ? 4 : 8;
+}
 static inline uint64_t raSortTiles(uint64_t slots) {
   const uint64_t tile = (uint64_t)RA_SORT_THREADS * raSortRounds(slots);
   return (slots + tile - 1) / tile;
 }
+// The next power of two of the number of experts.
+static inline __host__ __device__ uint32_t raSortWidth(int nExperts) { return nExperts <= 1 ? 1 : 1u << (32 - __builtin_clz((unsigned)nExperts - 1)); }
+// Every tile adds up the counts of all tiles by itself where that is at most 16 steps of its threads; otherwise a launch
+// between the two does it once (524288 slots of 384 experts: 30.2 us without it, 19.1 with it; of 128 experts 16.0 and 17.4).
+static inline bool raSortScanned(uint64_t tiles, int nExperts) { return tiles > 1 && tiles * raSortWidth(nExperts) > 16 * RA_SORT_THREADS; }
 hipError_t raLaunchSort(const RaSortArgs& a, hipStream_t s);
 
 #define RA_ROWS_MAX_TOPK 64
