@@ -1,7 +1,7 @@
 """A training step of two ranks (both on GPU 0, one process) through the collectives and the local operators together:
 a layer of experts, half of them on each rank, over all-gather and reduce-scatter, forward and backward, and then the clipped
 AdamW step of a sharded parameter between reduce-scatter and all-gather.  Checked against numpy in 64 bits.  Run by
-tests/test_gpu_shard_step.py in a process of its own: the communicators' windows live until it ends."""
+tests/test_gpu_kernels_step.py in a process of its own: the communicators' windows live until it ends."""
 import math
 import os
 import sys

@@ -1,4 +1,7 @@
-"""Token slots sorted by expert, rows dispatched and combined, and the gradients, against references in 64 bits."""
+"""Token slots sorted by expert, rows dispatched and combined, and the gradients, against references in 64 bits.
+
+Runs in the test runner's own process, which thereby opens the GPU; the name sorts behind test_gpu_fullsize, whose beds use
+sixteen processes of their own."""
 import numpy as np
 import pytest
 
