@@ -288,7 +288,8 @@ ncclResult_t rcclAmdNoAllocAsyncError(int device, ncclResult_t* asyncError);
 /* How AdamW's two moments are held.  rcclAmdStateF32: expAvg = m and expAvgSq = v as floats.
  * rcclAmdStateMx8: expAvg holds m and expAvgSq holds sqrt(v) in OCP MX blocks: each 32 consecutive elements of a tensor
  * (the last block may be shorter) are OCP e4m3 bytes (torch.float8_e4m3fn; not the encoding of ncclFp8E4M3) and share one
- * scale byte X with the value 2^(X-127) in expAvgScale / expAvgSqScale.  All zero bytes are the initial state. */
+ * scale byte X with the value 2^(X-127) in expAvgScale / expAvgSqScale (X = 0 counts as zero).  All zero bytes are the
+ * initial state. */
 typedef enum { rcclAmdStateF32 = 0, rcclAmdStateMx8 = 1 } rcclAmdStateType_t;
 #define RCCL_AMD_STATE_BLOCK 32
 
@@ -306,10 +307,10 @@ typedef struct {
 
 typedef struct {
   double lr, beta1, beta2, eps, weightDecay;
-  double gradScale;          /* gradients are multiplied by this first (1 / loss scale, 1 / ranks) */
+  double gradScale;          /* gradients are multiplied by this first (1 / loss scale, 1 / ranks); not negative */
   double maxNorm;            /* with sumSq: gradients are scaled down to this norm where theirs is larger */
   int64_t step;              /* 1 in the first step */
-  const int64_t* stepPtr;    /* device, or NULL: read by the kernel instead of `step` (for captured calls) */
+  const int64_t* stepPtr;    /* device, or NULL: read by the kernel instead of `step` (for captured calls); below 1 it counts as 1 */
   const float* lrPtr;        /* device, or NULL: read by the kernel instead of `lr` */
   const double* sumSq;       /* device, or NULL: no clipping.  The sum of squares of the unscaled gradients, of all ranks */
   uint64_t seed;             /* rcclAmdStateMx8: of the random bits with which the moments are rounded */
@@ -352,7 +353,8 @@ ncclResult_t rcclAmdExpertSort(const void* experts, ncclDataType_t expertType, s
 ncclResult_t rcclAmdExpertSortBytes(size_t tokens, int topk, int nExperts, size_t* workspaceBytes);
 
 /* Token rows in expert order: out[position[t * topk + k]] = x[t].  Rows of `hidden` elements, `xStride` and `outStride`
- * elements apart; `out` has `rows` rows, and positions outside 0 .. rows - 1 are passed over.  With offsets and counts
+ * elements apart; `out` has `rows` rows, and positions outside 0 .. rows - 1 are passed over.  Two slots may not name the
+ * same row.  With offsets and counts
  * (both or neither, as rcclAmdExpertSort gives them) the padding rows offsets[e] + counts[e] .. offsets[e + 1] - 1 are set to
  * zero; all other rows without a slot are left as they were.  Its gradient with respect to x is rcclAmdExpertCombine of
  * the gradient of out, without weights. */

@@ -257,23 +257,25 @@ template <typename T>
 __global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES void raLocalKernelDispatch(RaRowsArgs a, uint32_t groups, uint32_t parts, size_t partElems) {
   constexpr int N = Pack<T>::N, U = 8;
   if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
-  const uint64_t unit = (uint64_t)blockIdx.x * (blockDim.x >> 6) + uniform(threadIdx.x >> 6);
-  const size_t slot = unit / parts;
-  if (slot >= a.tokens * a.topk) return;
-  const int32_t pos = a.position[slot];
-  if (pos < 0 || (size_t)pos >= a.rows) return;
-  const T* x = (const T*)a.in + slot / a.topk * a.inStride;
-  T* out = (T*)a.out + (size_t)pos * a.outStride;
-  const size_t begin = unit % parts * partElems, end = begin + partElems < a.hidden ? begin + partElems : a.hidden;
-  size_t at = begin + (threadIdx.x & 63) * N;
-  for (; at + (U - 1) * 64 * N + N <= end; at += U * 64 * N) {
-    u32x4 p[U];
+  const uint32_t waves = blockDim.x >> 6;
+  const uint64_t units = (uint64_t)a.tokens * a.topk * parts;
+  for (uint64_t unit = (uint64_t)blockIdx.x * waves + uniform(threadIdx.x >> 6); unit < units; unit += (uint64_t)groups * waves) {
+    const size_t slot = unit / parts;
+    const int32_t pos = a.position[slot];
+    if (pos < 0 || (size_t)pos >= a.rows) continue;
+    const T* x = (const T*)a.in + slot / a.topk * a.inStride;
+    T* out = (T*)a.out + (size_t)pos * a.outStride;
+    const size_t begin = unit % parts * partElems, end = begin + partElems < a.hidden ? begin + partElems : a.hidden;
+    size_t at = begin + (threadIdx.x & 63) * N;
+    for (; at + (U - 1) * 64 * N + N <= end; at += U * 64 * N) {
+      u32x4 p[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) p[u] = wholePack<false>(x + at + u * 64 * N);
+      for (int u = 0; u < U; u++) p[u] = wholePack<false>(x + at + u * 64 * N);
 #pragma unroll
-    for (int u = 0; u < U; u++) storeWhole<false>(out + at + u * 64 * N, p[u]);
+      for (int u = 0; u < U; u++) storeWhole<false>(out + at + u * 64 * N, p[u]);
+    }
+    for (; at < end; at += 64 * N) storePack<false>(out, at, end, loadPack<false>(x, at, end));
   }
-  for (; at < end; at += 64 * N) storePack<false>(out, at, end, loadPack<false>(x, at, end));
 }
 
 // Combine.  A wave takes 64 * U packs of one token's row and adds those of its slots in the order of k, F rows in flight; the
@@ -325,20 +327,22 @@ template <typename T>
 __global__ __launch_bounds__(RA_COMBINE_THREADS) void raLocalKernelCombine(RaRowsArgs a, uint32_t parts, size_t partElems) {
   constexpr int N = Pack<T>::N, U = 4;
   const int lane = threadIdx.x & 63;
-  const uint64_t unit = (uint64_t)blockIdx.x * (RA_COMBINE_THREADS / 64) + uniform(threadIdx.x >> 6);
-  const size_t token = unit / parts;
-  if (token >= a.tokens) return;
-  int32_t pos = -1;
-  float w = 1.f;
-  if (lane < a.topk) {
-    pos = a.position[token * a.topk + lane];
-    if (a.weightType >= 0) w = weightOf(a.weights, a.weightType, token * a.topk + lane);
+  const uint64_t units = (uint64_t)a.tokens * parts;
+  for (uint64_t unit = (uint64_t)blockIdx.x * (RA_COMBINE_THREADS / 64) + uniform(threadIdx.x >> 6); unit < units;
+       unit += (uint64_t)gridDim.x * (RA_COMBINE_THREADS / 64)) {
+    const size_t token = unit / parts;
+    int32_t pos = -1;
+    float w = 1.f;
+    if (lane < a.topk) {
+      pos = a.position[token * a.topk + lane];
+      if (a.weightType >= 0) w = weightOf(a.weights, a.weightType, token * a.topk + lane);
+    }
+    const uint64_t slots = __ballot(pos >= 0 && (size_t)pos < a.rows);
+    size_t at = unit % parts * partElems;
+    const size_t end = at + partElems < a.hidden ? at + partElems : a.hidden;
+    for (; at + U * 64 * N <= end; at += U * 64 * N) combineAt<T, U, true>(a, token, at + lane * N, slots, pos, w);
+    for (; at < end; at += 64 * N) combineAt<T, 1, false>(a, token, at + lane * N, slots, pos, w);
   }
-  const uint64_t slots = __ballot(pos >= 0 && (size_t)pos < a.rows);
-  size_t at = unit % parts * partElems;
-  const size_t end = at + partElems < a.hidden ? at + partElems : a.hidden;
-  for (; at + U * 64 * N <= end; at += U * 64 * N) combineAt<T, U, true>(a, token, at + lane * N, slots, pos, w);
-  for (; at < end; at += 64 * N) combineAt<T, 1, false>(a, token, at + lane * N, slots, pos, w);
 }
 
 // The sum of x over the wave, in lane 63: inside rows of 16 lanes, then rows 0 and 2 into 1 and 3, then 1 into 3 (DPP moves).
@@ -370,34 +374,36 @@ template <typename T>
 __global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES void raLocalKernelCombineBackward(RaRowsArgs a, uint32_t groups) {
   constexpr int N = Pack<T>::N, U = 8;
   if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
-  const size_t slot = (size_t)blockIdx.x * (blockDim.x >> 6) + uniform(threadIdx.x >> 6);
-  if (slot >= a.tokens * a.topk) return;
-  const int32_t pos = a.position[slot];
-  float dot = 0.f;
-  if (pos >= 0 && (size_t)pos < a.rows) {
-    const float w = weightOf(a.weights, a.weightType, slot);
-    const T* dy = (const T*)a.in + slot / a.topk * a.inStride;
-    const T* z = (const T*)a.z + (size_t)pos * a.zStride;
-    T* dz = (T*)a.out + (size_t)pos * a.outStride;
-    size_t at = (threadIdx.x & 63) * N;
-    for (; at + (U - 1) * 64 * N + N <= a.hidden; at += U * 64 * N) {
-      u32x4 p[U], q[U];
+  const uint32_t waves = blockDim.x >> 6;
+  const size_t slots = a.tokens * a.topk;
+  for (size_t slot = (size_t)blockIdx.x * waves + uniform(threadIdx.x >> 6); slot < slots; slot += (size_t)groups * waves) {
+    const int32_t pos = a.position[slot];
+    float dot = 0.f;
+    if (pos >= 0 && (size_t)pos < a.rows) {
+      const float w = weightOf(a.weights, a.weightType, slot);
+      const T* dy = (const T*)a.in + slot / a.topk * a.inStride;
+      const T* z = (const T*)a.z + (size_t)pos * a.zStride;
+      T* dz = (T*)a.out + (size_t)pos * a.outStride;
+      size_t at = (threadIdx.x & 63) * N;
+      for (; at + (U - 1) * 64 * N + N <= a.hidden; at += U * 64 * N) {
+        u32x4 p[U], q[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) { p[u] = wholePack<true>(z + at + u * 64 * N); q[u] = wholePack<false>(dy + at + u * 64 * N); }
+        for (int u = 0; u < U; u++) { p[u] = wholePack<true>(z + at + u * 64 * N); q[u] = wholePack<false>(dy + at + u * 64 * N); }
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        storeWhole<true>(dz + at + u * 64 * N, gradients<T>(p[u], q[u], w, dot));
-        __builtin_amdgcn_sched_barrier(0);                 // one pack as floats at a time: the packs take half of the registers
+        for (int u = 0; u < U; u++) {
+          storeWhole<true>(dz + at + u * 64 * N, gradients<T>(p[u], q[u], w, dot));
+          __builtin_amdgcn_sched_barrier(0);               // one pack as floats at a time: the packs take half of the registers
+        }
       }
+      for (; at < a.hidden; at += 64 * N)
+        storePack<true>(dz, at, a.hidden, gradients<T>(loadPack<true>(z, at, a.hidden), loadPack<false>(dy, at, a.hidden), w, dot));
+      dot = waveSum63(dot);
     }
-    for (; at < a.hidden; at += 64 * N)
-      storePack<true>(dz, at, a.hidden, gradients<T>(loadPack<true>(z, at, a.hidden), loadPack<false>(dy, at, a.hidden), w, dot));
-    dot = waveSum63(dot);
-  }
-  if ((threadIdx.x & 63) == 63) {
-    if (a.weightType == ncclFloat32) ((float*)a.dweights)[slot] = dot;
-    else if (a.weightType == ncclBfloat16) ((__bf16*)a.dweights)[slot] = (__bf16)dot;
-    else ((_Float16*)a.dweights)[slot] = (_Float16)dot;
+    if ((threadIdx.x & 63) == 63) {
+      if (a.weightType == ncclFloat32) ((float*)a.dweights)[slot] = dot;
+      else if (a.weightType == ncclBfloat16) ((__bf16*)a.dweights)[slot] = (__bf16)dot;
+      else ((_Float16*)a.dweights)[slot] = (_Float16)dot;
+    }
   }
 }
 
@@ -405,7 +411,12 @@ static uint32_t padGroups(const RaRowsArgs& a) { return a.offsets ? (uint32_t)a.
 
 // Threads of a workgroup of slots: whole tokens, eight waves or nearly so.
 static int slotThreads(int topk) { return 64 * (topk <= 8 ? 8 / topk * topk : topk <= 16 ? topk : 8); }
-static uint64_t groupsOf(uint64_t units, int threads) { return (units + threads / 64 - 1) / (threads / 64); }
+// Workgroups for so many waves: one each, up to 2^20 workgroups, beyond which a wave takes several in turn (a launch has fewer
+// than 2^32 threads).
+static uint32_t groupsOf(uint64_t units, int threads) {
+  const uint64_t g = (units + threads / 64 - 1) / (threads / 64);
+  return (uint32_t)(g < 1u << 20 ? g : 1u << 20);
+}
 
 template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_t s) {
   const uint64_t slots = (uint64_t)a.tokens * a.topk, step = 64 * Pack<T>::N;
@@ -415,26 +426,23 @@ template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_
   const size_t partElems = ((a.hidden + parts - 1) / parts + step - 1) / step * step;
   parts = (a.hidden + partElems - 1) / partElems;
   const int threads = slotThreads(a.topk);
-  const uint64_t groups = groupsOf(slots * parts, threads);
-  if (groups + padGroups(a) > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const uint32_t groups = groupsOf(slots * parts, threads);
   if (groups + padGroups(a) == 0) return hipSuccess;
-  hipLaunchKernelGGL(raLocalKernelDispatch<T>, dim3((uint32_t)groups + padGroups(a)), dim3(threads), 0, s, a, (uint32_t)groups, (uint32_t)parts, partElems);
+  hipLaunchKernelGGL(raLocalKernelDispatch<T>, dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups, (uint32_t)parts, partElems);
   return hipGetLastError();
 }
 template <typename T> static hipError_t combine(const RaRowsArgs& a, hipStream_t s) {
   const uint64_t step = 64 * Pack<T>::N;
   // four runs of 64 packs for each wave, or one where that leaves fewer than 4096 waves
   const size_t partElems = a.tokens * ((a.hidden + 4 * step - 1) / (4 * step)) < 4096 ? step : 4 * step;
-  const uint64_t parts = (a.hidden + partElems - 1) / partElems, groups = groupsOf(a.tokens * parts, RA_COMBINE_THREADS);
-  if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(raLocalKernelCombine<T>, dim3((uint32_t)groups), dim3(RA_COMBINE_THREADS), 0, s, a, (uint32_t)parts, partElems);
+  const uint64_t parts = (a.hidden + partElems - 1) / partElems;
+  hipLaunchKernelGGL(raLocalKernelCombine<T>, dim3(groupsOf(a.tokens * parts, RA_COMBINE_THREADS)), dim3(RA_COMBINE_THREADS), 0, s, a, (uint32_t)parts, partElems);
   return hipGetLastError();
 }
 template <typename T> static hipError_t combineBackward(const RaRowsArgs& a, hipStream_t s) {
   const int threads = slotThreads(a.topk);
-  const uint64_t groups = groupsOf((uint64_t)a.tokens * a.topk, threads);
-  if (groups + padGroups(a) > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((raLocalKernelCombineBackward<T>), dim3((uint32_t)groups + padGroups(a)), dim3(threads), 0, s, a, (uint32_t)groups);
+  const uint32_t groups = groupsOf((uint64_t)a.tokens * a.topk, threads);
+  hipLaunchKernelGGL((raLocalKernelCombineBackward<T>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups);
   return hipGetLastError();
 }
 #define RA_BY_TYPE(fn)                                    \

@@ -228,7 +228,7 @@ __global__ __launch_bounds__(RA_ADAMW_THREADS) __attribute__((amdgpu_waves_per_e
   Scalars s = {a.b1, a.omb1, a.b2, a.omb2, a.eps, a.decay, a.stepSize, a.rootC2, a.coef};
   int64_t step = a.step;
   if (a.stepPtr || a.lrPtr) {
-    if (a.stepPtr) step = *a.stepPtr;
+    if (a.stepPtr) step = *a.stepPtr > 1 ? *a.stepPtr : 1;
     const double lr = a.lrPtr ? (double)*a.lrPtr : a.lr;
     s.decay = uniform((float)(1.0 - lr * a.weightDecay));
     s.stepSize = uniform((float)(lr / (1.0 - powN(a.beta1, step))));

@@ -69,7 +69,8 @@ RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntenso
   if (!isFloat(paramType) || !isFloat(gradType)) RA_REFUSE("%s: parameter type %d / gradient type %d is not float32, bfloat16 or float16", fn, (int)paramType, (int)gradType);
   if (stateType != rcclAmdStateF32 && stateType != rcclAmdStateMx8) RA_REFUSE("%s: unknown state type %d", fn, (int)stateType);
   const rcclAmdAdamWConfig_t& c = *config;
-  if (!isfinite(c.lr) || !isfinite(c.weightDecay) || !isfinite(c.gradScale) || !isfinite(c.eps) || c.eps < 0.0) RA_REFUSE("%s: lr, weightDecay, gradScale and eps must be finite, eps not negative", fn);
+  if (!isfinite(c.lr) || !isfinite(c.weightDecay) || !isfinite(c.gradScale) || !isfinite(c.eps) || c.eps < 0.0 || c.gradScale < 0.0)
+    RA_REFUSE("%s: lr, weightDecay, gradScale and eps must be finite, gradScale and eps not negative", fn);
   if (!(c.beta1 >= 0.0 && c.beta1 < 1.0 && c.beta2 >= 0.0 && c.beta2 < 1.0)) RA_REFUSE("%s: beta1 = %g, beta2 = %g outside 0 <= beta < 1", fn, c.beta1, c.beta2);
   if (!c.stepPtr && c.step < 1) RA_REFUSE("%s: step %lld: the first step is 1", fn, (long long)c.step);
   if (c.sumSq && !(c.maxNorm >= 0.0)) RA_REFUSE("%s: maxNorm %g with sumSq", fn, c.maxNorm);
@@ -115,6 +116,7 @@ RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntenso
     if (elements == 0) continue;
     uint64_t chunk = mx ? (elements / 4096 + unit - 1) / unit * unit : unit;
     chunk = chunk < unit ? unit : chunk > 4 * unit ? 4 * unit : chunk;
+    while (elements / chunk > 1u << 22) chunk *= 2;       // (a launch has fewer than 2^32 threads)
     for (int i = 0; i < n; i++) {
       const rcclAmdAdamWTensor_t& t = tensors[lo + i];
       if (flat) {

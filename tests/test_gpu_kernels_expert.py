@@ -248,10 +248,9 @@ def test_combine_backward(tokens, topk, hidden, dtype, gap, shift, weights, in_p
     keep = r.used | r.pad
     assert np.all(np.abs(got[keep] - want[keep]) <= bound[keep])
     assert np.array_equal(got[~keep], want[~keep], equal_nan=True)
-    # dw: a lane adds at most 16 products to a sum for each part of the row that a workgroup takes (16384 elements or more,
-    # or the whole row), then 6 + 16 sums join them; the largest row here has 3 parts
+    # dw: a lane adds the products of its part of the row (a 64th of it, in packs of at most 8 elements), then 6 sums join them
     halfw = ref.HALF_STEP[weights] if weights != "f32" else 0.0
-    bound = 1.01 * (3 * 16 + 3 + 22) * ref.U * size
+    bound = 1.01 * (hidden // 64 + 8 + 6) * ref.U * size
     bound += halfw * (np.abs(want_w) + bound) + ref.TINY[weights]
     assert np.all(np.abs(_np64(dw) - want_w) <= bound)
     assert _outside(flat, dz, before)
@@ -337,6 +336,29 @@ def test_large_rows_pass_32_bits_of_offset():
     w, dw = torch.full((tokens, 1), 2.0, device="cuda"), torch.empty(tokens, 1, device="cuda")
     ra.expert_combine_backward(x, out, rows, w, ra.ncclFloat32, out, dw, ra.ncclBfloat16, tokens, 1, hidden, pos)
     assert torch.equal(out[rows - tokens:], 2 * x)
+
+
+def test_more_slots_than_a_launch_has_waves():
+    """72 million slots of eight elements, moved by a permutation: a wave takes several slots."""
+    import torch
+    import rccl_amd as ra
+    tokens, topk, hidden = 9_000_001, 8, 8
+    rows = tokens * topk
+    gen = torch.Generator("cuda").manual_seed(1)
+    pos = torch.randperm(rows, device="cuda", generator=gen).to(torch.int32)
+    x = torch.randint(-4, 5, (tokens, hidden), device="cuda", generator=gen).to(torch.bfloat16)
+    out = torch.zeros(rows, hidden, dtype=torch.bfloat16, device="cuda")
+    ra.expert_dispatch(x, out, rows, ra.ncclBfloat16, tokens, topk, hidden, pos)
+    want = torch.empty_like(out)
+    want[pos.long()] = x.repeat_interleave(topk, 0)
+    assert torch.equal(out, want)
+    y = torch.empty_like(x)
+    ra.expert_combine(out, rows, None, -1, y, ra.ncclBfloat16, tokens, topk, hidden, pos)
+    assert torch.equal(y, topk * x)
+    w, dw = torch.full((tokens, topk), 2.0, device="cuda"), torch.empty(tokens, topk, device="cuda")
+    ra.expert_combine_backward(x, out, rows, w, ra.ncclFloat32, out, dw, ra.ncclBfloat16, tokens, topk, hidden, pos)
+    assert torch.equal(out, 2 * want)
+    assert torch.equal(dw, x.float().square().sum(1, keepdim=True).expand(tokens, topk))
 
 
 def test_no_tokens():

@@ -362,6 +362,21 @@ def test_sum_squares(dtype, shift):
         assert float(out) == first + first
 
 
+def test_sum_squares_past_32_bits_of_elements():
+    import torch
+    import rccl_amd as ra
+    n = 2 ** 32 + 2 ** 31 + 5
+    if torch.cuda.mem_get_info()[0] < 20 * 2 ** 30:
+        pytest.skip("needs 20 GiB of free device memory")
+    x = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    for i, v in ((0, 1.0), (2 ** 31 - 1, 2.0), (2 ** 31, 3.0), (2 ** 32 - 1, 4.0), (2 ** 32, 5.0), (2 ** 32 + 2 ** 31, 6.0), (n - 1, 7.0)):
+        x[i] = v
+    out = torch.zeros(1, dtype=torch.float64, device="cuda")
+    work = torch.empty(ra.sum_squares_bytes(2), dtype=torch.uint8, device="cuda")
+    ra.sum_squares([x, x[:0]], None, ra.ncclBfloat16, out, work)
+    assert float(out) == 1 + 4 + 9 + 16 + 25 + 36 + 49
+
+
 def test_sum_squares_of_large_values_does_not_overflow():
     import torch
     import rccl_amd as ra
@@ -429,6 +444,63 @@ def test_step_and_rate_from_the_device(mx):
                 assert torch.all((x.double() - y.double()).abs() <= 8 * ref.U * (x.double().abs() + old.abs()))
             else:
                 assert torch.equal(x, y)
+
+
+def test_step_number_below_one_counts_as_one():
+    import torch
+    a, b = (Case([100], "f32", "f32", None, seed=36) for _ in range(2))
+    a.run(step=1)
+    b.run(step_ptr=torch.tensor([-3], dtype=torch.int64, device="cuda"))
+    assert torch.equal(a.param, b.param)
+
+
+@pytest.mark.parametrize("layout", ["flat", "scattered", "mixed copies", "reversed"])
+@pytest.mark.parametrize("mx", [False, True])
+def test_layouts_of_many_tensors(layout, mx):
+    """Tensors that lie alike in flat buffers take one kind of launch, any others another: the results are the same bits."""
+    import torch
+    import rccl_amd as ra
+    rng = np.random.default_rng(7)
+    sizes = [int(x) for x in rng.integers(0, 300, 400)]
+    a, b = (Case(sizes, "f32", "bf16", "bf16", mx=mx, seed=37) for _ in range(2))
+    ty = _types()
+
+    def run(case, table):
+        ra.adamw(table, ty["f32"][0], ty["bf16"][0], ty["bf16"][0], ra.rcclAmdStateMx8 if mx else ra.rcclAmdStateF32, seed=5, **HYPER)
+
+    ta, tb = a.table(), b.table()
+    run(a, ta)
+    order = np.arange(len(sizes))
+    keep = []
+    if layout == "scattered":                       # one gradient of a tensor lies elsewhere
+        i = next(i for i in range(100, 400) if sizes[i] > 10)
+        keep.append(b.cut(b.grad, i).clone())
+        tb[i, 1] = keep[0].data_ptr()
+    elif layout == "mixed copies":
+        skip = [i for i in range(len(sizes)) if i % 3 == 0]
+        tb[skip, 6] = 0
+        for i in skip:
+            b.cut(b.copy, i).copy_(a.cut(a.copy, i))
+    elif layout == "reversed":                      # (the place of a tensor in the call is part of its random bits)
+        order = order[::-1]
+        if mx:
+            tb = tb[order]
+            before = b.snapshot()
+            run(b, tb)
+            f = [order.tolist().index(i) for i in range(len(sizes))]
+            for i in range(0, len(sizes), 37):
+                n = sizes[i]
+                old = {id(x): o for x, o in zip(b.bufs, before)}
+                g = b.cut(b.grad, i).float().cpu().numpy()
+                m0 = _f32(ref.mx_decode(_np(b.cut(old[id(b.m)], i)), _np(b.cut_scale(old[id(b.ms)], i))))
+                m = np.float32(HYPER["beta1"]) * m0 + np.float32(1 - HYPER["beta1"]) * g
+                bits = ref.hash32(5, HYPER["step"], f[i], np.arange(n, dtype=np.uint64))
+                code, scale = ref.mx_encode(m, (bits & np.uint64(0xFFFF)).astype(np.int64), False)
+                assert np.array_equal(_np(b.cut(b.m, i)), code) and np.array_equal(_np(b.cut_scale(b.ms, i)), scale)
+            return
+    run(b, tb[order])
+    for x, y in zip(a.bufs, b.bufs):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), layout
 
 
 @pytest.mark.parametrize("mx", [False, True])

@@ -25,7 +25,7 @@ def _adamw(rows=None, **kw):
 
 @pytest.mark.parametrize("kw,text", [
     (dict(param_type=ra.ncclFloat64), "parameter type"), (dict(grad_type=ra.ncclInt32), "gradient type"), (dict(state_type=2), "state type"),
-    (dict(lr=float("nan")), "finite"), (dict(eps=-1.0), "eps"), (dict(weight_decay=float("inf")), "finite"), (dict(grad_scale=float("nan")), "finite"),
+    (dict(lr=float("nan")), "finite"), (dict(eps=-1.0), "eps"), (dict(weight_decay=float("inf")), "finite"), (dict(grad_scale=float("nan")), "finite"), (dict(grad_scale=-1.0), "negative"),
     (dict(beta1=1.0), "beta1"), (dict(beta2=-0.1), "beta"), (dict(beta2=float("nan")), "beta"), (dict(step=0), "first step"),
     (dict(sum_sq=P, max_norm=-1.0), "maxNorm"), (dict(sum_sq=P, max_norm=float("nan")), "maxNorm"), (dict(sum_sq=P + 4), "misaligned"), (dict(step_ptr=P + 2), "misaligned"),
     (dict(rows=[[0, P, P, P, 0, 0, 0, 1]]), "null buffer"), (dict(rows=[[P, P, P, 0, 0, 0, 0, 1]]), "null buffer"),
