@@ -228,6 +228,11 @@ static __device__ __forceinline__ float weightOf(const void* w, int type, size_t
   if (type == ncclBfloat16) return (float)((const __bf16*)w)[i];
   return (float)((const _Float16*)w)[i];
 }
+static __device__ __forceinline__ void storeWeight(void* w, int type, size_t i, float x) {
+  if (type == ncclFloat32) ((float*)w)[i] = x;
+  else if (type == ncclBfloat16) ((__bf16*)w)[i] = (__bf16)x;
+  else ((_Float16*)w)[i] = (_Float16)x;
+}
 // Lane k of the wave holds what belongs to slot k of its token.
 static __device__ __forceinline__ int laneInt(int x, int k) { return __builtin_amdgcn_readlane(x, k); }
 static __device__ __forceinline__ float laneFloat(float x, int k) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), k)); }
@@ -245,46 +250,113 @@ template <typename T> static __device__ __forceinline__ void padRows(const RaRow
       storePack<false>((T*)a.out + (size_t)row * a.outStride, at, a.hidden, u32x4{0, 0, 0, 0});
 }
 
-// Dispatch.  A wave takes one slot's row (or a part of it, where there are too few slots to fill the GPU), 8 packs in flight
-// for each lane: long runs of one row are what the time follows here.  16384 tokens of 8 slots, 4096 bf16 elements (1.24 GB
-// to move): 8 KiB in one go 0.220 ms, 4 KiB 0.225, 2 KiB 0.235; a wave that reads a row once and writes all of the token's
-// rows 0.236; streaming accesses 0.225 to 0.250.  The waves of a token's slots are in one workgroup, so that its row comes
-// from HBM once.  Sixteen waves of a compute unit at a time (RA_FEW_WAVES): with 20, 24 and 32 the runs of more rows mix, and
-// the time is 0.226, 0.239 and 0.244 ms.
+// How a row is cut: `head` single elements up to the first 16-byte boundary of the row that is written, then `body`
+// elements in packs, then single ones again.  Stores of 16 bytes that are not aligned cost up to half of the bandwidth,
+// loads that are not cost little.  The at most 14 single elements are one access of a wave: see elementOf.
+struct RowCut { uint32_t head, body, single; };         // single = hidden - body
+template <typename T> static __device__ __forceinline__ RowCut cutRow(const T* out, size_t hidden) {
+  constexpr uint32_t N = Pack<T>::N;
+  uint32_t head = (uint32_t)((16 - ((uintptr_t)out & 15)) & 15) / (uint32_t)sizeof(T);
+  if (head > hidden) head = (uint32_t)hidden;
+  const uint32_t body = ((uint32_t)hidden - head) / N * N;
+  return RowCut{head, body, (uint32_t)hidden - body};
+}
+// Which element is a lane's single one, of `singles` in the row.
+static __device__ __forceinline__ uint32_t elementOf(uint32_t head, size_t hidden, uint32_t singles, uint32_t lane) { return lane < head ? lane : (uint32_t)hidden - singles + lane; }
+
+// Dispatch.  A wave takes S slots at a time, V = 8 / S packs in flight for each lane and slot: one slot with rows over 256
+// packs (parts of a row, where there are too few slots to fill the GPU), more with shorter ones.  Long runs of one row are what the
+// time follows: 16384 tokens of 8 slots, 4096 bf16 elements (1.24 GB to move): 8 KiB in one go 0.220 ms, 4 KiB 0.225, 2 KiB
+// 0.235; a wave that reads a row once and writes all of the token's rows 0.236, the same through LDS 0.236; streaming accesses
+// 0.225 to 0.250.  The waves of a token's slots are in one workgroup, so that its row comes from HBM once.
 #define RA_SLOT_THREADS 1024         // at most; see slotThreads
-#define RA_FEW_WAVES __attribute__((amdgpu_waves_per_eu(4, 4)))
-template <typename T>
-__global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES void raLocalKernelDispatch(RaRowsArgs a, uint32_t groups, uint32_t parts, size_t partElems) {
-  constexpr int N = Pack<T>::N, U = 8;
+// Sixteen waves of a compute unit at a time: with 20, 24 and 32 the runs of more rows mix, and the time is 0.226, 0.239 and 0.244 ms.
+#define RA_FEW_WAVES(most) __attribute__((amdgpu_waves_per_eu(4, most)))
+template <typename T, int S>
+__global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES(S == 1 ? 4 : 8) void raLocalKernelDispatch(RaRowsArgs a, uint32_t groups, uint32_t parts, uint32_t partElems) {
+  constexpr uint32_t N = Pack<T>::N, U = 8, V = S == 1 ? 4 : U / S;      // V: packs of a slot in what is left of its row
   if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
-  const uint32_t waves = blockDim.x >> 6;
-  const uint64_t units = (uint64_t)a.tokens * a.topk * parts;
+  const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  const size_t slots = a.tokens * a.topk;
+  const uint64_t units = S == 1 ? slots * parts : (slots + S - 1) / S;
   for (uint64_t unit = (uint64_t)blockIdx.x * waves + uniform(threadIdx.x >> 6); unit < units; unit += (uint64_t)groups * waves) {
-    const size_t slot = unit / parts;
-    const int32_t pos = a.position[slot];
-    if (pos < 0 || (size_t)pos >= a.rows) continue;
-    const T* x = (const T*)a.in + slot / a.topk * a.inStride;
-    T* out = (T*)a.out + (size_t)pos * a.outStride;
-    const size_t begin = unit % parts * partElems, end = begin + partElems < a.hidden ? begin + partElems : a.hidden;
-    size_t at = begin + (threadIdx.x & 63) * N;
-    for (; at + (U - 1) * 64 * N + N <= end; at += U * 64 * N) {
-      u32x4 p[U];
+    const size_t slot = S == 1 ? unit / parts : unit * S;
+    const T* x[S];
+    T* out[S];
+    RowCut c[S];
+    bool go[S];
 #pragma unroll
-      for (int u = 0; u < U; u++) p[u] = wholePack<false>(x + at + u * 64 * N);
-#pragma unroll
-      for (int u = 0; u < U; u++) storeWhole<false>(out + at + u * 64 * N, p[u]);
+    for (int s = 0; s < S; s++) {
+      const int32_t pos = slot + s < slots ? a.position[slot + s] : -1;
+      go[s] = pos >= 0 && (size_t)pos < a.rows;
+      x[s] = (const T*)a.in + (size_t)((uint32_t)(slot + s) / (uint32_t)a.topk) * a.inStride;
+      out[s] = (T*)a.out + (size_t)(go[s] ? pos : 0) * a.outStride;
+      c[s] = cutRow(out[s], a.hidden);
     }
-    for (; at < end; at += 64 * N) storePack<false>(out, at, end, loadPack<false>(x, at, end));
+    uint32_t run = 0;
+    if (S == 1) {
+      if (!go[0]) continue;
+      const uint32_t part = (uint32_t)(unit % parts);
+      run = part * partElems;
+      if (part) c[0].single = 0;                           // (the single elements go with the first part)
+      if (run + partElems < c[0].body) c[0].body = run + partElems;
+    }
+    for (; S == 1 && run + U * 64 * N <= c[0].body; run += U * 64 * N) {
+      u32x4 p[U];
+      const T* from = x[0] + c[0].head + run + lane * N;
+      T* to = out[0] + c[0].head + run + lane * N;
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++) p[u] = wholePack<false>(from + u * 64 * N);
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++) storeWhole<false>(to + u * 64 * N, p[u]);
+    }
+    T single[S];
+    if (S == 1 && lane < c[0].single) single[0] = x[0][elementOf(c[0].head, a.hidden, c[0].single, lane)];
+    do {
+      u32x4 p[S][V];
+#pragma unroll
+      for (int s = 0; s < S; s++) {
+        const T* from = x[s] + c[s].head + run + lane * N;
+#pragma unroll
+        for (uint32_t v = 0; v < V; v++) if (go[s] && run + (v * 64 + lane) * N < c[s].body) p[s][v] = wholePack<false>(from + v * 64 * N);
+        if (S > 1 && go[s] && lane < c[s].single) single[s] = x[s][elementOf(c[s].head, a.hidden, c[s].single, lane)];
+      }
+#pragma unroll
+      for (int s = 0; s < S; s++) {
+        T* to = out[s] + c[s].head + run + lane * N;
+#pragma unroll
+        for (uint32_t v = 0; v < V; v++) if (go[s] && run + (v * 64 + lane) * N < c[s].body) storeWhole<false>(to + v * 64 * N, p[s][v]);
+        if (S > 1 && go[s] && lane < c[s].single) out[s][elementOf(c[s].head, a.hidden, c[s].single, lane)] = single[s];
+      }
+      run += V * 64 * N;
+    } while (S == 1 && run < c[0].body);
+    if (S == 1 && lane < c[0].single) out[0][elementOf(c[0].head, a.hidden, c[0].single, lane)] = single[0];
   }
 }
 
-// Combine.  A wave takes 64 * U packs of one token's row and adds those of its slots in the order of k, F rows in flight; the
-// part in which a row ends, and all of it where there are few tokens, in runs of 64 packs.  The same micro-batch back (1.21 GB):
+// Rows of at most 32 packs: a group of `1 << shift` lanes takes one, so that a wave moves several at a time.
+#define RA_NARROW_THREADS 256
+template <typename T>
+__global__ __launch_bounds__(RA_NARROW_THREADS) void raLocalKernelDispatchNarrow(RaRowsArgs a, uint32_t groups, uint32_t shift) {
+  constexpr int N = Pack<T>::N;
+  if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
+  const size_t slots = a.tokens * a.topk, step = (size_t)groups * RA_NARROW_THREADS >> shift;
+  const size_t at = (threadIdx.x & ((1u << shift) - 1)) * N;
+  for (size_t slot = ((size_t)blockIdx.x * RA_NARROW_THREADS + threadIdx.x) >> shift; slot < slots; slot += step) {
+    const int32_t pos = a.position[slot];
+    if (pos < 0 || (size_t)pos >= a.rows || at >= a.hidden) continue;
+    storePack<false>((T*)a.out + (size_t)pos * a.outStride, at, a.hidden, loadPack<false>((const T*)a.in + (size_t)((uint32_t)slot / (uint32_t)a.topk) * a.inStride, at, a.hidden));
+  }
+}
+
+// Combine.  A wave takes 64 * U packs of one token's row (64 where there are few tokens) and adds those of its slots in the order
+// of k, F rows in flight.  The same micro-batch back (1.21 GB):
 // U = 4 and F = 4 0.205 ms, U = 2 0.209, U = 4 and F = 2 0.206 (F = 8 0.202, but with more registers than eight waves of a
 // compute unit's SIMD have), accesses that are not streaming 0.235.
 #define RA_COMBINE_THREADS 256
+// WHOLE: all of the packs at element `at` + ... exist; otherwise those before `end` do.
 template <typename T, int U, bool WHOLE>
-static __device__ __forceinline__ void combineAt(const RaRowsArgs& a, size_t token, size_t at, uint64_t slots, int32_t pos, float w) {
+static __device__ __forceinline__ void combineAt(const RaRowsArgs& a, T* y, uint32_t at, uint32_t end, uint64_t slots, int32_t pos, float w) {
   constexpr int N = Pack<T>::N, F = 4;
   typedef typename Pack<T>::floats floats;
   floats sum[U];
@@ -303,7 +375,7 @@ static __device__ __forceinline__ void combineAt(const RaRowsArgs& a, size_t tok
       wk[f] = laneFloat(w, k);
       const T* z = (const T*)a.in + (size_t)laneInt(pos, k) * a.inStride;
 #pragma unroll
-      for (int u = 0; u < U; u++) p[f][u] = WHOLE ? wholePack<true>(z + at + u * 64 * N) : loadPack<true>(z, at + u * 64 * N, a.hidden);
+      for (int u = 0; u < U; u++) if (WHOLE || at + u * 64 * N < end) p[f][u] = wholePack<true>(z + at + u * 64 * N); else p[f][u] = u32x4{0, 0, 0, 0};
     }
 #pragma unroll
     for (int f = 0; f < F; f++) {
@@ -316,32 +388,86 @@ static __device__ __forceinline__ void combineAt(const RaRowsArgs& a, size_t tok
       }
     }
   }
-  T* y = (T*)a.out + token * a.outStride;
 #pragma unroll
-  for (int u = 0; u < U; u++) {
-    if (WHOLE) storeWhole<true>(y + at + u * 64 * N, fromFloats<T>(sum[u]));
-    else storePack<true>(y, at + u * 64 * N, a.hidden, fromFloats<T>(sum[u]));
+  for (int u = 0; u < U; u++) if (WHOLE || at + u * 64 * N < end) storeWhole<true>(y + at + u * 64 * N, fromFloats<T>(sum[u]));
+}
+// The same for one element of each lane.
+template <typename T> static __device__ __forceinline__ void combineElement(const RaRowsArgs& a, T* y, uint32_t at, uint64_t slots, int32_t pos, float w) {
+  constexpr int F = 8;
+  float sum = 0.f;
+  while (slots) {
+    float z[F], wk[F];
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      z[f] = wk[f] = 0.f;
+      if (!slots) continue;
+      const int k = __builtin_ctzll(slots);
+      slots &= slots - 1;
+      wk[f] = laneFloat(w, k);
+      z[f] = (float)((const T*)a.in)[(size_t)laneInt(pos, k) * a.inStride + at];
+    }
+#pragma unroll
+    for (int f = 0; f < F; f++) sum = __builtin_fmaf(wk[f], z[f], sum);      // (a slot that is not there adds 0 * 0)
   }
+  y[at] = (T)sum;
 }
 template <typename T>
-__global__ __launch_bounds__(RA_COMBINE_THREADS) void raLocalKernelCombine(RaRowsArgs a, uint32_t parts, size_t partElems) {
-  constexpr int N = Pack<T>::N, U = 4;
-  const int lane = threadIdx.x & 63;
+__global__ __launch_bounds__(RA_COMBINE_THREADS) void raLocalKernelCombine(RaRowsArgs a, uint32_t parts, uint32_t partElems) {
+  constexpr uint32_t N = Pack<T>::N, U = 4;
+  const uint32_t lane = threadIdx.x & 63;
   const uint64_t units = (uint64_t)a.tokens * parts;
   for (uint64_t unit = (uint64_t)blockIdx.x * (RA_COMBINE_THREADS / 64) + uniform(threadIdx.x >> 6); unit < units;
        unit += (uint64_t)gridDim.x * (RA_COMBINE_THREADS / 64)) {
     const size_t token = unit / parts;
     int32_t pos = -1;
     float w = 1.f;
-    if (lane < a.topk) {
+    if (lane < (uint32_t)a.topk) {
       pos = a.position[token * a.topk + lane];
       if (a.weightType >= 0) w = weightOf(a.weights, a.weightType, token * a.topk + lane);
     }
     const uint64_t slots = __ballot(pos >= 0 && (size_t)pos < a.rows);
-    size_t at = unit % parts * partElems;
-    const size_t end = at + partElems < a.hidden ? at + partElems : a.hidden;
-    for (; at + U * 64 * N <= end; at += U * 64 * N) combineAt<T, U, true>(a, token, at + lane * N, slots, pos, w);
-    for (; at < end; at += 64 * N) combineAt<T, 1, false>(a, token, at + lane * N, slots, pos, w);
+    T* y = (T*)a.out + token * a.outStride;
+    const RowCut c = cutRow(y, a.hidden);
+    const uint32_t run = (uint32_t)(unit % parts) * partElems;
+    const uint32_t at = c.head + run + lane * N, end = c.head + (run + partElems < c.body ? run + partElems : c.body);
+    if (partElems == 64 * N) combineAt<T, 1, false>(a, y, at, end, slots, pos, w);
+    else if (c.head + run + U * 64 * N <= end) combineAt<T, U, true>(a, y, at, end, slots, pos, w);
+    else combineAt<T, U, false>(a, y, at, end, slots, pos, w);
+    if (run == 0 && lane < c.single) combineElement(a, y, elementOf(c.head, a.hidden, c.single, lane), slots, pos, w);
+  }
+}
+
+// Rows of at most 32 packs: `1 << shift` lanes for each token.
+template <typename T>
+__global__ __launch_bounds__(RA_NARROW_THREADS) void raLocalKernelCombineNarrow(RaRowsArgs a, uint32_t shift) {
+  constexpr int N = Pack<T>::N, F = 4;
+  typedef typename Pack<T>::floats floats;
+  const size_t step = (size_t)gridDim.x * RA_NARROW_THREADS >> shift, at = (threadIdx.x & ((1u << shift) - 1)) * N;
+  if (at >= a.hidden) return;
+  for (size_t token = ((size_t)blockIdx.x * RA_NARROW_THREADS + threadIdx.x) >> shift; token < a.tokens; token += step) {
+    floats sum = {};
+    for (int k = 0; k < a.topk; k += F) {
+      u32x4 p[F];
+      float w[F];
+#pragma unroll
+      for (int f = 0; f < F; f++) {
+        p[f] = u32x4{0, 0, 0, 0};
+        w[f] = 0.f;
+        if (k + f >= a.topk) continue;
+        const size_t slot = token * a.topk + k + f;
+        const int32_t pos = a.position[slot];
+        if (pos < 0 || (size_t)pos >= a.rows) continue;
+        w[f] = a.weightType >= 0 ? weightOf(a.weights, a.weightType, slot) : 1.f;
+        p[f] = loadPack<true>((const T*)a.in + (size_t)pos * a.inStride, at, a.hidden);
+      }
+#pragma unroll
+      for (int f = 0; f < F; f++) {                        // (a slot that is not there adds 0 * 0)
+        const floats z = toFloats<T>(p[f]);
+#pragma unroll
+        for (int i = 0; i < N; i++) sum[i] = __builtin_fmaf(w[f], z[i], sum[i]);
+      }
+    }
+    storePack<true>((T*)a.out + token * a.outStride, at, a.hidden, fromFloats<T>(sum));
   }
 }
 
@@ -367,43 +493,103 @@ template <typename T> static __device__ __forceinline__ u32x4 gradients(u32x4 z,
   return fromFloats<T>(g);
 }
 
-// The gradients of combine.  A wave takes one slot: dz's row is written while z's row passes, and their product stays in the
-// wave.  Runs of 8 KiB as in dispatch: half of the slots of 16384 tokens (1.23 GB) 0.232 ms, runs of 4 KiB 0.240, 2 KiB 0.243; a
-// workgroup for each token, its row in registers, 0.234 at best.
-template <typename T>
-__global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES void raLocalKernelCombineBackward(RaRowsArgs a, uint32_t groups) {
-  constexpr int N = Pack<T>::N, U = 8;
+// The gradients of combine.  A wave takes S slots: dz's rows are written while z's rows pass, and their products stay in the
+// wave.  Runs of 8 KiB as in dispatch: half of the slots of 16384 tokens (1.17 to 1.38 GB, as routing goes) 6.0 to 6.1 TB/s, a copy
+// has 6.3; runs of 4 KiB 3 % slower, 2 KiB 5 %; a workgroup for each token, its row in registers, no faster.
+template <typename T, int S>
+__global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES(S == 1 ? 4 : 8) void raLocalKernelCombineBackward(RaRowsArgs a, uint32_t groups) {
+  constexpr uint32_t N = Pack<T>::N, V = S == 1 ? 4 : 4 / S;      // packs of a slot in what is left of its row
   if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
-  const uint32_t waves = blockDim.x >> 6;
+  const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63;
   const size_t slots = a.tokens * a.topk;
-  for (size_t slot = (size_t)blockIdx.x * waves + uniform(threadIdx.x >> 6); slot < slots; slot += (size_t)groups * waves) {
-    const int32_t pos = a.position[slot];
-    float dot = 0.f;
-    if (pos >= 0 && (size_t)pos < a.rows) {
-      const float w = weightOf(a.weights, a.weightType, slot);
-      const T* dy = (const T*)a.in + slot / a.topk * a.inStride;
-      const T* z = (const T*)a.z + (size_t)pos * a.zStride;
-      T* dz = (T*)a.out + (size_t)pos * a.outStride;
-      size_t at = (threadIdx.x & 63) * N;
-      for (; at + (U - 1) * 64 * N + N <= a.hidden; at += U * 64 * N) {
+  for (size_t slot = ((size_t)blockIdx.x * waves + uniform(threadIdx.x >> 6)) * S; slot < slots; slot += (size_t)groups * waves * S) {
+    const T* dy[S];
+    const T* z[S];
+    T* dz[S];
+    RowCut c[S];
+    bool go[S];
+    float w[S], dot[S];
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      const bool exists = slot + s < slots;
+      const int32_t pos = exists ? a.position[slot + s] : -1;
+      go[s] = pos >= 0 && (size_t)pos < a.rows;
+      w[s] = go[s] ? weightOf(a.weights, a.weightType, slot + s) : 0.f;
+      dot[s] = 0.f;
+      const size_t row = go[s] ? pos : 0;
+      dy[s] = (const T*)a.in + (size_t)((uint32_t)(slot + s) / (uint32_t)a.topk) * a.inStride;
+      z[s] = (const T*)a.z + row * a.zStride;
+      dz[s] = (T*)a.out + row * a.outStride;
+      c[s] = cutRow(dz[s], a.hidden);
+    }
+    uint32_t run = 0;
+    if (S == 1 && go[0]) {
+      constexpr uint32_t U = 8;
+      for (; run + U * 64 * N <= c[0].body; run += U * 64 * N) {
+        const uint32_t at = c[0].head + run + lane * N;
         u32x4 p[U], q[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) { p[u] = wholePack<true>(z + at + u * 64 * N); q[u] = wholePack<false>(dy + at + u * 64 * N); }
+        for (uint32_t u = 0; u < U; u++) { p[u] = wholePack<true>(z[0] + at + u * 64 * N); q[u] = wholePack<false>(dy[0] + at + u * 64 * N); }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          storeWhole<true>(dz + at + u * 64 * N, gradients<T>(p[u], q[u], w, dot));
+        for (uint32_t u = 0; u < U; u++) {
+          storeWhole<true>(dz[0] + at + u * 64 * N, gradients<T>(p[u], q[u], w[0], dot[0]));
           __builtin_amdgcn_sched_barrier(0);               // one pack as floats at a time: the packs take half of the registers
         }
       }
-      for (; at < a.hidden; at += 64 * N)
-        storePack<true>(dz, at, a.hidden, gradients<T>(loadPack<true>(z, at, a.hidden), loadPack<false>(dy, at, a.hidden), w, dot));
-      dot = waveSum63(dot);
     }
-    if ((threadIdx.x & 63) == 63) {
-      if (a.weightType == ncclFloat32) ((float*)a.dweights)[slot] = dot;
-      else if (a.weightType == ncclBfloat16) ((__bf16*)a.dweights)[slot] = (__bf16)dot;
-      else ((_Float16*)a.dweights)[slot] = (_Float16)dot;
+    do {
+      u32x4 p[S][V], q[S][V];
+#pragma unroll
+      for (int s = 0; s < S; s++) {
+        const uint32_t at = c[s].head + run + lane * N;
+#pragma unroll
+        for (uint32_t v = 0; v < V; v++)
+          if (go[s] && run + (v * 64 + lane) * N < c[s].body) { p[s][v] = wholePack<true>(z[s] + at + v * 64 * N); q[s][v] = wholePack<false>(dy[s] + at + v * 64 * N); }
+      }
+#pragma unroll
+      for (int s = 0; s < S; s++) {
+        const uint32_t at = c[s].head + run + lane * N;
+#pragma unroll
+        for (uint32_t v = 0; v < V; v++)
+          if (go[s] && run + (v * 64 + lane) * N < c[s].body) storeWhole<true>(dz[s] + at + v * 64 * N, gradients<T>(p[s][v], q[s][v], w[s], dot[s]));
+      }
+      run += V * 64 * N;
+    } while (S == 1 && go[0] && run < c[0].body);
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      if (go[s] && lane < c[s].single) {
+        const uint32_t i = elementOf(c[s].head, a.hidden, c[s].single, lane);
+        const float d = (float)dy[s][i];
+        dot[s] = __builtin_fmaf(d, (float)z[s][i], dot[s]);
+        dz[s][i] = (T)(w[s] * d);
+      }
     }
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      const float sum = waveSum63(dot[s]);
+      if (lane == 63 && slot + s < slots) storeWeight(a.dweights, a.weightType, slot + s, sum);
+    }
+  }
+}
+
+// Rows of at most 32 packs: `1 << shift` lanes for each slot.
+template <typename T>
+__global__ __launch_bounds__(RA_NARROW_THREADS) void raLocalKernelCombineBackwardNarrow(RaRowsArgs a, uint32_t groups, uint32_t shift) {
+  constexpr int N = Pack<T>::N;
+  if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
+  const size_t slots = a.tokens * a.topk, step = (size_t)groups * RA_NARROW_THREADS >> shift;
+  const size_t at = (threadIdx.x & ((1u << shift) - 1)) * N;
+  for (size_t slot = ((size_t)blockIdx.x * RA_NARROW_THREADS + threadIdx.x) >> shift; slot < slots; slot += step) {
+    const int32_t pos = a.position[slot];
+    float dot = 0.f;
+    if (pos >= 0 && (size_t)pos < a.rows && at < a.hidden) {
+      const float w = weightOf(a.weights, a.weightType, slot);
+      const u32x4 d = loadPack<false>((const T*)a.in + (size_t)((uint32_t)slot / (uint32_t)a.topk) * a.inStride, at, a.hidden);
+      const u32x4 z = loadPack<true>((const T*)a.z + (size_t)pos * a.zStride, at, a.hidden);
+      storePack<true>((T*)a.out + (size_t)pos * a.outStride, at, a.hidden, gradients<T>(z, d, w, dot));
+    }
+    for (int s = 1; s < 1 << shift; s <<= 1) dot += __shfl_xor(dot, s);      // (the lanes of a slot run together)
+    if (at == 0) storeWeight(a.dweights, a.weightType, slot, dot);
   }
 }
 
@@ -418,31 +604,70 @@ static uint32_t groupsOf(uint64_t units, int threads) {
   return (uint32_t)(g < 1u << 20 ? g : 1u << 20);
 }
 
-template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_t s) {
-  const uint64_t slots = (uint64_t)a.tokens * a.topk, step = 64 * Pack<T>::N;
-  // parts of a row, down to 64 packs, where there are fewer than 4096 waves otherwise
-  uint64_t parts = 1, most = (a.hidden + step - 1) / step;
-  while (parts < most && slots * parts < 4096) parts *= 2;
-  const size_t partElems = ((a.hidden + parts - 1) / parts + step - 1) / step * step;
-  parts = (a.hidden + partElems - 1) / partElems;
-  const int threads = slotThreads(a.topk);
-  const uint32_t groups = groupsOf(slots * parts, threads);
-  if (groups + padGroups(a) == 0) return hipSuccess;
-  hipLaunchKernelGGL(raLocalKernelDispatch<T>, dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups, (uint32_t)parts, partElems);
+// Lanes for a row of few packs, as a power of two; 6 (a whole wave): the row is not narrow.
+template <typename T> static uint32_t narrowShift(const RaRowsArgs& a) {
+  uint32_t shift = 0;
+  while (shift < 6 && ((uint64_t)Pack<T>::N << shift) < a.hidden) shift++;
+  return shift;
+}
+template <typename T, int S>
+static hipError_t launchDispatch(const RaRowsArgs& a, uint32_t groups, int threads, uint32_t parts, uint32_t partElems, hipStream_t s) {
+  if (groups + padGroups(a)) hipLaunchKernelGGL((raLocalKernelDispatch<T, S>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups, parts, partElems);
   return hipGetLastError();
 }
+template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_t s) {
+  const uint32_t shift = narrowShift<T>(a);
+  if (shift < 6) {
+    const uint32_t groups = groupsOf(((uint64_t)a.tokens * a.topk + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS);
+    if (groups + padGroups(a)) hipLaunchKernelGGL(raLocalKernelDispatchNarrow<T>, dim3(groups + padGroups(a)), dim3(RA_NARROW_THREADS), 0, s, a, groups, shift);
+    return hipGetLastError();
+  }
+  const uint64_t slots = (uint64_t)a.tokens * a.topk, step = 64 * Pack<T>::N;
+  const int threads = slotThreads(a.topk);
+  // Short rows: several slots for a wave, where that leaves 4096 waves
+  const uint64_t runs = (a.hidden + step - 1) / step;
+  if (runs <= 1 && slots >= 8 * 4096) return launchDispatch<T, 8>(a, groupsOf((slots + 7) / 8, threads), threads, 1, 0, s);
+  if (runs <= 2 && slots >= 4 * 4096) return launchDispatch<T, 4>(a, groupsOf((slots + 3) / 4, threads), threads, 1, 0, s);
+  if (runs <= 4 && slots >= 2 * 4096) return launchDispatch<T, 2>(a, groupsOf((slots + 1) / 2, threads), threads, 1, 0, s);
+  // parts of a row, down to 64 packs, where there are fewer than 4096 waves otherwise
+  uint64_t parts = 1;
+  while (parts < runs && slots * parts < 4096) parts *= 2;
+  const uint64_t partElems = ((a.hidden + parts - 1) / parts + step - 1) / step * step;
+  parts = (a.hidden + partElems - 1) / partElems;
+  return launchDispatch<T, 1>(a, groupsOf(slots * parts, threads), threads, (uint32_t)parts, (uint32_t)partElems, s);
+}
 template <typename T> static hipError_t combine(const RaRowsArgs& a, hipStream_t s) {
+  const uint32_t shift = narrowShift<T>(a);
+  if (shift < 6) {
+    hipLaunchKernelGGL(raLocalKernelCombineNarrow<T>, dim3(groupsOf((a.tokens + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS)), dim3(RA_NARROW_THREADS), 0, s, a, shift);
+    return hipGetLastError();
+  }
   const uint64_t step = 64 * Pack<T>::N;
   // four runs of 64 packs for each wave, or one where that leaves fewer than 4096 waves
   const size_t partElems = a.tokens * ((a.hidden + 4 * step - 1) / (4 * step)) < 4096 ? step : 4 * step;
   const uint64_t parts = (a.hidden + partElems - 1) / partElems;
-  hipLaunchKernelGGL(raLocalKernelCombine<T>, dim3(groupsOf(a.tokens * parts, RA_COMBINE_THREADS)), dim3(RA_COMBINE_THREADS), 0, s, a, (uint32_t)parts, partElems);
+  hipLaunchKernelGGL(raLocalKernelCombine<T>, dim3(groupsOf(a.tokens * parts, RA_COMBINE_THREADS)), dim3(RA_COMBINE_THREADS), 0, s, a, (uint32_t)parts, (uint32_t)partElems);
   return hipGetLastError();
 }
 template <typename T> static hipError_t combineBackward(const RaRowsArgs& a, hipStream_t s) {
+  const uint32_t shift = narrowShift<T>(a);
+  if (shift < 6) {
+    const uint32_t groups = groupsOf(((uint64_t)a.tokens * a.topk + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS);
+    hipLaunchKernelGGL(raLocalKernelCombineBackwardNarrow<T>, dim3(groups + padGroups(a)), dim3(RA_NARROW_THREADS), 0, s, a, groups, shift);
+    return hipGetLastError();
+  }
   const int threads = slotThreads(a.topk);
-  const uint32_t groups = groupsOf((uint64_t)a.tokens * a.topk, threads);
-  hipLaunchKernelGGL((raLocalKernelCombineBackward<T>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups);
+  const uint64_t slots = (uint64_t)a.tokens * a.topk, runs = (a.hidden + 64 * Pack<T>::N - 1) / (64 * Pack<T>::N);
+  if (runs <= 1 && slots >= 4096 * 4) {
+    const uint32_t groups = groupsOf((slots + 3) / 4, threads);
+    hipLaunchKernelGGL((raLocalKernelCombineBackward<T, 4>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups);
+  } else if (runs <= 2 && slots >= 4096 * 2) {
+    const uint32_t groups = groupsOf((slots + 1) / 2, threads);
+    hipLaunchKernelGGL((raLocalKernelCombineBackward<T, 2>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups);
+  } else {
+    const uint32_t groups = groupsOf(slots, threads);
+    hipLaunchKernelGGL((raLocalKernelCombineBackward<T, 1>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups);
+  }
   return hipGetLastError();
 }
 #define RA_BY_TYPE(fn)                                    \

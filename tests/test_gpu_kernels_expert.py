@@ -256,6 +256,63 @@ def test_combine_backward(tokens, topk, hidden, dtype, gap, shift, weights, in_p
     assert _outside(flat, dz, before)
 
 
+@pytest.mark.parametrize("topk,tokens", [(8, 4500), (3, 11000), (1, 33000)])
+@pytest.mark.parametrize("hidden,dtype,gap,shift", [(129, "f32", 0, 0), (257, "bf16", 0, 0), (400, "f16", 1, 3), (512, "bf16", 0, 0), (513, "bf16", 2, 1), (300, "f32", 1, 1),
+                                                    (1023, "f16", 0, 5), (1024, "bf16", 8, 0), (1030, "bf16", 1, 0), (520, "f32", 0, 2), (2047, "bf16", 0, 0), (1024, "f32", 3, 0)])
+def test_short_rows_of_many_slots(topk, tokens, hidden, dtype, gap, shift):
+    """Rows of one to four KiB in so many slots that a wave takes several of them; a reference in 64 bits on the GPU."""
+    import torch
+    import rccl_amd as ra
+    gen = torch.Generator("cuda").manual_seed(hidden + topk)
+    code, tt = _types()[dtype]
+    pos = torch.full((tokens * topk,), -1, dtype=torch.int64, device="cuda")
+    keep = torch.rand(tokens * topk, device="cuda", generator=gen) < 0.9
+    held = int(keep.sum())
+    rows = held + 37                                    # the last ones belong to nobody
+    pos[keep] = torch.randperm(held + 20, device="cuda", generator=gen)[:held]
+    used = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    used[pos[keep]] = True
+    pos32 = pos.to(torch.int32)
+    wide = hidden + gap
+
+    def matrix(r, fill=None):
+        flat = torch.randn((r + 2) * wide + 64, device="cuda", generator=gen).to(tt) if fill is None else torch.full(((r + 2) * wide + 64,), fill, dtype=tt, device="cuda")
+        return flat, flat[wide + shift:wide + shift + r * wide].view(r, wide)[:, :hidden]
+
+    _, x = matrix(tokens)
+    flat, out = matrix(rows, 5.0)
+    before = flat.clone()
+    ra.expert_dispatch(x, out, rows, code, tokens, topk, hidden, pos32)
+    token = torch.arange(tokens * topk, device="cuda") // topk
+    want = torch.full((rows, hidden), 5.0, dtype=tt, device="cuda")
+    want[pos[keep]] = x[token[keep]]
+    assert torch.equal(out, want) and _outside(flat, out, before)
+
+    _, z = matrix(rows)
+    z[~used] = float("nan")
+    w = torch.randn(tokens, topk, device="cuda", generator=gen)
+    flat, y = matrix(tokens, 5.0)
+    before = flat.clone()
+    ra.expert_combine(z, rows, w, ra.ncclFloat32, y, code, tokens, topk, hidden, pos32)
+    zg = torch.where(keep[:, None], z[pos.clamp(min=0)].double(), 0.0).view(tokens, topk, hidden)
+    terms = zg * w.double()[:, :, None]
+    half = ref.HALF_STEP[dtype] if dtype != "f32" else 0.0
+    bound = 1.01 * topk * ref.U * terms.abs().sum(1)
+    bound += half * (terms.sum(1).abs() + bound) + ref.TINY[dtype]
+    assert torch.all((y.double() - terms.sum(1)).abs() <= bound) and _outside(flat, y, before)
+
+    _, dy = matrix(tokens)
+    flat, dz = matrix(rows, 5.0)
+    before = flat.clone()
+    dw = torch.full((tokens, topk), 9.0, device="cuda")
+    ra.expert_combine_backward(dy, z, rows, w, ra.ncclFloat32, dz, dw, code, tokens, topk, hidden, pos32)
+    want = torch.full((rows, hidden), 5.0, dtype=torch.float64, device="cuda")
+    want[pos[keep]] = dy[token[keep]].double() * w.double().view(-1)[keep, None]
+    assert torch.all((dz.double() - want).abs() <= (1.01 * ref.U + 1.01 * half) * want.abs() + ref.TINY[dtype]) and _outside(flat, dz, before)
+    prod = zg * dy.double()[:, None, :]
+    assert torch.all((dw.double() - prod.sum(2)).abs() <= 1.01 * (hidden // 64 + 14) * ref.U * prod.abs().sum(2) + ref.TINY["f32"])
+
+
 def test_gradients_against_differences():
     """<dy, combine(z, w)> is linear in z and in w: its differences are exact up to rounding, in fp32 with small whole numbers
     exactly.  The gradient of a dispatch is a combine without weights: <dout, dispatch(x)> = <combine(dout), x>."""
