@@ -73,10 +73,10 @@ static __device__ __forceinline__ double powN(double x, int64_t n) {
 struct Scalars { float b1, omb1, b2, omb2, eps, decay, stepSize, rootC2, coef; };
 
 // ------------------------------------------------------------------ 8-bit states
+static __device__ __forceinline__ float powerOf(uint32_t scale) { return __uint_as_float(scale << 23); }      // 2^(X-127)
 static __device__ __forceinline__ f32x4 decode4(uint32_t code, uint32_t scale) {
-  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, true);
-  const float f = __uint_as_float(scale << 23);          // 2^(X-127); 0 for X = 0, which only an all-zero block has
-  return f32x4{lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f};
+  const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, powerOf(scale), false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, powerOf(scale), true);
+  return f32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 static __device__ __forceinline__ uint32_t maxOf8(uint32_t a) {      // over the 8 lanes that hold a block, with DPP moves
   uint32_t o;
@@ -89,24 +89,15 @@ static __device__ __forceinline__ uint32_t scaleOf(uint32_t most) {
   const int x = (int)((most + 0x1FFFFFu) >> 23) - 8;
   return (uint32_t)(x < 1 ? 1 : x > 247 ? 247 : x);
 }
-// Stochastic rounding to the e4m3 grid.  y is the scaled value, rnd 20 random bits: they are added below the third bit of
-// the mantissa and what is below it is cut off.  Values under 2^-6 are moved to the binade above first, whose grid of 2^-9
-// is that of e4m3's subnormal numbers.  The result is a value of the grid, so the conversion that follows is exact.
-template <bool KEEP> static __device__ __forceinline__ float roundRandom(float y, uint32_t rnd) {
-  const float a = __builtin_fabsf(y);
-  const float low = a < 0x1p-6f ? 0x1p-6f : 0.f;
-  float c = __uint_as_float((__float_as_uint(a + low) + rnd) & 0xFFF00000u) - low;
-  if (KEEP && y > 0.f) c = c > 0x1p-9f ? c : 0x1p-9f;    // a second moment over zero stays over zero
-  c = __builtin_copysignf(c, y);
-  return a < __builtin_inff() ? c : __builtin_nanf("");
-}
-template <bool KEEP> static __device__ __forceinline__ uint32_t encode4(f32x4 x, uint32_t scale, const uint32_t (&rnd)[4]) {
-  const float inv = __uint_as_float((254u - scale) << 23);
-  float y[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) y[i] = roundRandom<KEEP>(x[i] * inv, rnd[i]);
-  int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
+// Stochastic rounding to the e4m3 grid, by the instruction for it: of x / scale, the 20 high bits of `rnd` are added below the
+// third bit of the mantissa (below 2^-9 in the subnormal range) and what is below it is cut off.  Values that are not
+// finite become NaN.  Written out in integer operations this took a third of the kernel's VALU time.
+static __device__ __forceinline__ uint32_t encode4(f32x4 x, uint32_t scale, const uint32_t (&rnd)[4]) {
+  const float f = powerOf(scale);
+  uint32_t c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(0, x[0], rnd[0], f, 0);
+  c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[1], rnd[1], f, 1);
+  c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[2], rnd[2], f, 2);
+  return __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[3], rnd[3], f, 3);
 }
 static __device__ __forceinline__ uint32_t bitsMax(f32x4 x) {
   uint32_t a = 0;
@@ -159,8 +150,10 @@ template <typename P, typename G, bool MX> struct Row {
     else if (copyType == ncclBfloat16) storeAs((__bf16*)copy + at, whole, left);
     else storeAs((_Float16*)copy + at, whole, left);
   }
-  // Division and square root are the correctly rounded ones; nothing is contracted, so that a rounding of an 8-bit state
-  // does not depend on how this is compiled.
+  // Square roots are the correctly rounded ones and nothing is contracted, so that a rounding of an 8-bit state does not depend
+  // on how this is compiled.  So is the quotient with fp32 states; with 8-bit states, where VALU time counts, it is a product
+  // with the reciprocal instruction's result, which is off by at most one unit of the last place.  The divisor is zero or
+  // above 2^-75 (a root of an fp32 number), far from where that instruction loses range.
   template <bool WHOLE> __device__ __forceinline__ void update(const Scalars& s, size_t at, int left, uint32_t key) {
     f32x4 r;
     if constexpr (MX) { fm = decode4(qm, xm); r = decode4(qv, xv); fv = r * r; }
@@ -170,7 +163,8 @@ template <typename P, typename G, bool MX> struct Row {
       fm[i] = s.b1 * fm[i] + s.omb1 * gi;
       fv[i] = s.b2 * fv[i] + s.omb2 * (gi * gi);
       r[i] = __builtin_sqrtf(fv[i]);
-      p[i] = p[i] * s.decay - s.stepSize * (fm[i] / (r[i] * s.rootC2 + s.eps));
+      const float down = r[i] * s.rootC2 + s.eps;
+      p[i] = p[i] * s.decay - s.stepSize * (MX ? fm[i] * __builtin_amdgcn_rcpf(down) : fm[i] / down);
     }
     const bool whole = WHOLE || left >= 4;
     storeAs(param + at, whole, left);
@@ -178,14 +172,16 @@ template <typename P, typename G, bool MX> struct Row {
     if constexpr (MX) {
       // (what does not exist is zero: its gradient and its moments were)
       const uint32_t em = scaleOf(maxOf8(bitsMax(fm))), ev = scaleOf(maxOf8(bitsMax(r)));
-      uint32_t rm[4], rv[4];
+      const float least = powerOf(ev) * 0x1p-9f;            // a second moment over zero stays over zero
+      uint32_t rm[4], rv[4];                                // 16 random bits, and a half of the last of them
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const uint32_t h = mix((uint32_t)at + (uint32_t)i + key);
-        rm[i] = (h & 0xFFFFu) << 4 | 8u;
-        rv[i] = (h >> 16) << 4 | 8u;
+        rm[i] = h << 16 | 0x8000u;
+        rv[i] = (h & 0xFFFF0000u) | 0x8000u;
+        if (r[i] > 0.f) r[i] = r[i] > least ? r[i] : least;
       }
-      const uint32_t nm = encode4<false>(fm, em, rm), nv = encode4<true>(r, ev, rv);
+      const uint32_t nm = encode4(fm, em, rm), nv = encode4(r, ev, rv);
       if (whole) { __builtin_nontemporal_store(nm, (u32_u*)(cm + at)); __builtin_nontemporal_store(nv, (u32_u*)(cv + at)); }
       else if (left > 0) {
         cm[at] = (uint8_t)nm; cv[at] = (uint8_t)nv;
