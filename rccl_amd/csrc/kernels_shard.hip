@@ -195,12 +195,13 @@ template <typename P, typename G, bool MX> struct Row {
 };
 
 template <typename P, typename G, bool MX>
-__global__ __launch_bounds__(RA_ADAMW_THREADS) __attribute__((amdgpu_waves_per_eu(1, MX ? 8 : 4))) void raLocalKernelAdamW(RaAdamWArgs a) {
-  // Rows in flight for each wave.  fp32 states: one, and one row for each wave in all, so that the workgroups that run at a
-  // time stream through one window of memory: a shard of 67 million elements (1.88 GB) 0.310 ms = 6.07 TB/s, and with 2, 4 and 16
-  // rows for each wave 0.313, 0.320 and 0.350; accesses that are not streaming 0.369.  8-bit states have 100 VALU cycles for
-  // each element, as long as memory takes, and a longer start: two rows at a time of four, 0.177 ms (1.08 GB, 6.1 TB/s).
-  // Of fp32 states no more than 16 waves run on a compute unit, which is 1.5 % faster than 32: fewer runs of memory at a time.
+__global__ __launch_bounds__(RA_ADAMW_THREADS) __attribute__((amdgpu_waves_per_eu(1, MX && sizeof(P) == 2 ? 8 : 4))) void raLocalKernelAdamW(RaAdamWArgs a) {
+  // Rows in flight for each wave, and no more than 16 waves on a compute unit, so that the workgroups that run at a time
+  // stream through one window of memory.  fp32 states: one row for each wave in all, a shard of 67 million elements (1.88 GB) 0.302 ms
+  // = 6.2 TB/s; with 2, 4 and 16 rows for each wave 0.313, 0.320 and 0.350, with 32 waves 0.311, with accesses that are not streaming
+  // 0.369.  8-bit states: two rows at once and in all (the start of a workgroup counts for more), 33.5 million elements of fp32
+  // (541 MB) 0.089 ms = 6.1 TB/s, of four rows 0.094; parameters in 16 bits, bound by their 60 VALU cycles for each element, four rows
+  // and 32 waves 0.062 (340 MB), of two rows 0.068.
   constexpr int U = MX ? 2 : 1;
   constexpr uint32_t STEP = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW;
   uint32_t t, chunk0;

@@ -106,16 +106,16 @@ RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntenso
   const bool flat = ntensors > general && liesFlat(tensors, ntensors, mx, ps, gs, cs, a.flat.base);
   const int fit = flat ? RA_ADAMW_FLAT : general;
   if (flat) a.stride = 0;
-  // A chunk is the work of one workgroup: four rows (1024 elements), or up to four times that for 8-bit states where there
-  // is much to do (see the kernel).
-  const uint64_t unit = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW;
+  // A chunk is the work of one workgroup: a row for each wave (1024 elements), with 8-bit states up to two, or four with
+  // parameters in 16 bits, where there is much to do (see the kernel).
+  const uint64_t unit = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW, most = ps == 4 ? 2 : 4;
   for (int lo = 0; lo < ntensors; lo += fit) {
     const int n = ntensors - lo < fit ? ntensors - lo : fit;
     uint64_t elements = 0, chunks = 0;
     for (int i = 0; i < n; i++) elements += tensors[lo + i].count;
     if (elements == 0) continue;
     uint64_t chunk = mx ? (elements / 4096 + unit - 1) / unit * unit : unit;
-    chunk = chunk < unit ? unit : chunk > 4 * unit ? 4 * unit : chunk;
+    chunk = chunk < unit ? unit : chunk > most * unit ? most * unit : chunk;
     while (elements / chunk > 1u << 22) chunk *= 2;       // (a launch has fewer than 2^32 threads)
     for (int i = 0; i < n; i++) {
       const rcclAmdAdamWTensor_t& t = tensors[lo + i];
