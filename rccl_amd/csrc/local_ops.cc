@@ -106,9 +106,9 @@ RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntenso
   const bool flat = ntensors > general && liesFlat(tensors, ntensors, mx, ps, gs, cs, a.flat.base);
   const int fit = flat ? RA_ADAMW_FLAT : general;
   if (flat) a.stride = 0;
-  // A chunk is the work of one workgroup: a row for each wave (1024 elements), with 8-bit states up to two, or four with
-  // parameters in 16 bits, where there is much to do (see the kernel).
-  const uint64_t unit = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW, most = ps == 4 ? 2 : 4;
+  // A chunk is the work of one workgroup: a row for each wave (1024 elements), with 8-bit states up to two, or four where
+  // parameter and gradient have 16 bits and there is no copy, where there is much to do (see the kernel).
+  const uint64_t unit = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW, most = ps + gs + (copies ? cs : 0) > 4 ? 2 : 4;
   for (int lo = 0; lo < ntensors; lo += fit) {
     const int n = ntensors - lo < fit ? ntensors - lo : fit;
     uint64_t elements = 0, chunks = 0;
