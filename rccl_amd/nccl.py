@@ -381,9 +381,12 @@ def reduce_copy(dst, srcs, count, datatype, op=ncclSum, stream=None):
 # A buffer is a device pointer (int) or a torch tensor.  A tensor is checked before its address is taken: on the current
 # device, of the element type the call names, and reaching as far as the call will.  Rows may be strided: the stride of a
 # two-dimensional tensor is taken from it.
+# Plain calls (contiguous tensors) go through a small CPython module, csrc/mirror.c, which makes the same checks and calls the
+# same functions in about half of the host's time; it answers -1 to what is not plain, and the way here says what is wrong.
 
 _TORCH = {}                                     # what the checks need of torch, looked up once: element types by their code
 _current_device = _current_stream = None
+_mirror = None                                  # the CPython module, once it knows torch and the library
 
 
 def _torch():
@@ -393,6 +396,22 @@ def _torch():
     _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
     _TORCH.update({ncclFloat32: torch.float32, ncclBfloat16: torch.bfloat16, ncclFloat16: torch.float16, ncclFloat64: torch.float64,
                    ncclInt32: torch.int32, ncclInt64: torch.int64})
+
+
+def _bind():
+    """The CPython module, with torch's types and the addresses of the library's functions."""
+    global _mirror
+    try:
+        from . import _mirror as module
+    except ImportError as e:
+        raise OSError(f"the module _mirror is missing ({e}): build it with `make -C rccl_amd/csrc -j8`") from e
+    if not _TORCH:
+        _torch()
+    L = lib()
+    module.bind(_TORCH, _current_device, _current_stream, tuple(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in (
+        "rcclAmdAdamW", "rcclAmdSumSquares", "rcclAmdExpertSort", "rcclAmdExpertDispatch", "rcclAmdExpertCombine", "rcclAmdExpertCombineBackward")))
+    _mirror = module
+    return module
 
 
 def _refuse(where, why):
@@ -503,6 +522,11 @@ def adamw(tensors, param_type, grad_type, copy_type=-1, state_type=rcclAmdStateF
     (the fields of rcclAmdAdamWTensor_t); a program whose buffers stay where they are keeps the table.  step_ptr (int64),
     lr_ptr (float32) and sum_sq (float64) are one-element device buffers that the kernel reads."""
     where = "rcclAmdAdamW"
+    if _mirror or not isinstance(stream, int):
+        rc = (_mirror or _bind()).adamw(tensors, param_type, grad_type, copy_type, state_type, lr, beta1, beta2, eps, weight_decay, step, step_ptr, lr_ptr,
+                                         grad_scale, sum_sq, max_norm, seed, stream)
+        if rc >= 0:
+            return _check(rc, where)
     rows, n, keep = _host_table(tensors, 8, where) if len(tensors) else (None, 0, None)
     c = rcclAmdAdamWConfig_t(lr, beta1, beta2, eps, weight_decay, grad_scale, max_norm, step, _whole(step_ptr, 1, ncclInt64, where, "step_ptr"),
                              _whole(lr_ptr, 1, ncclFloat32, where, "lr_ptr"), _whole(sum_sq, 1, ncclFloat64, where, "sum_sq"), seed & 0xFFFFFFFFFFFFFFFF)
@@ -521,6 +545,10 @@ def sum_squares(tensors, counts, datatype, out, workspace, accumulate=False, str
     """rcclAmdSumSquares: out[0] (float64) = sum of the squares of all elements.  `tensors`: a list of torch tensors (counts
     may be None) or an array of device addresses, `counts` an array of their sizes."""
     where = "rcclAmdSumSquares"
+    if _mirror or not isinstance(stream, int):
+        rc = (_mirror or _bind()).sum_squares(tensors, counts, datatype, out, workspace, accumulate, stream)
+        if rc >= 0:
+            return _check(rc, where)
     if isinstance(tensors, (list, tuple)) and tensors and hasattr(tensors[0], "data_ptr"):
         counts = [t.numel() for t in tensors] if counts is None else counts
         tensors = [_whole(t, n, datatype, where, "a tensor") for t, n in zip(tensors, counts)]
@@ -549,6 +577,10 @@ def expert_sort(experts, expert_type, tokens, topk, first_expert, n_experts, row
                 workspace=None, stream=None):
     """rcclAmdExpertSort: rows of the slots in the order of the experts first_expert .. first_expert + n_experts - 1."""
     where = "rcclAmdExpertSort"
+    if _mirror or not isinstance(stream, int):
+        rc = (_mirror or _bind()).expert_sort(experts, expert_type, tokens, topk, first_expert, n_experts, row_align, position, source, offsets, counts, workspace, stream)
+        if rc >= 0:
+            return _check(rc, where)
     slots = tokens * topk
     w, nbytes = _work(workspace, expert_sort_bytes(tokens, topk, n_experts) if isinstance(workspace, int) else 0, where)
     _check(lib().rcclAmdExpertSort(_whole(experts, slots, expert_type, where, "experts"), expert_type, tokens, topk, first_expert, n_experts, row_align,
@@ -561,6 +593,10 @@ def expert_sort(experts, expert_type, tokens, topk, first_expert, n_experts, row
 def expert_dispatch(x, out, rows, datatype, tokens, topk, hidden, position, offsets=None, counts=None, n_experts=0, x_stride=None, out_stride=None, stream=None):
     """rcclAmdExpertDispatch: out[position[t, k]] = x[t]; its gradient is expert_combine of out's without weights."""
     where = "rcclAmdExpertDispatch"
+    if x_stride is None and out_stride is None and (_mirror or not isinstance(stream, int)):
+        rc = (_mirror or _bind()).expert_dispatch(x, out, rows, datatype, tokens, topk, hidden, position, offsets, counts, n_experts, stream)
+        if rc >= 0:
+            return _check(rc, where)
     x, xs = _matrix(x, x_stride, tokens, hidden, datatype, where, "x")
     out, os_ = _matrix(out, out_stride, rows, hidden, datatype, where, "out")
     _check(lib().rcclAmdExpertDispatch(x, xs, out, os_, rows, datatype, tokens, topk, hidden, _whole(position, tokens * topk, ncclInt32, where, "position"),
@@ -571,6 +607,10 @@ def expert_dispatch(x, out, rows, datatype, tokens, topk, hidden, position, offs
 def expert_combine(z, rows, weights, weight_type, y, datatype, tokens, topk, hidden, position, z_stride=None, y_stride=None, stream=None):
     """rcclAmdExpertCombine: y[t] = sum over k of weights[t, k] * z[position[t, k]]; weights None: all ones."""
     where = "rcclAmdExpertCombine"
+    if z_stride is None and y_stride is None and (_mirror or not isinstance(stream, int)):
+        rc = (_mirror or _bind()).expert_combine(z, rows, weights, weight_type, y, datatype, tokens, topk, hidden, position, stream)
+        if rc >= 0:
+            return _check(rc, where)
     z, zs = _matrix(z, z_stride, rows, hidden, datatype, where, "z")
     y, ys = _matrix(y, y_stride, tokens, hidden, datatype, where, "y")
     _check(lib().rcclAmdExpertCombine(z, zs, rows, _whole(weights, tokens * topk, weight_type, where, "weights"), weight_type, y, ys, datatype, tokens, topk, hidden,
@@ -581,6 +621,11 @@ def expert_combine_backward(dy, z, rows, weights, weight_type, dz, dweights, dat
                             dy_stride=None, z_stride=None, dz_stride=None, stream=None):
     """rcclAmdExpertCombineBackward: dz[position[t, k]] = weights[t, k] * dy[t], dweights[t, k] = <dy[t], z[position[t, k]]>."""
     where = "rcclAmdExpertCombineBackward"
+    if dy_stride is None and z_stride is None and dz_stride is None and (_mirror or not isinstance(stream, int)):
+        rc = (_mirror or _bind()).expert_combine_backward(dy, z, rows, weights, weight_type, dz, dweights, datatype, tokens, topk, hidden, position, offsets, counts,
+                                                           n_experts, stream)
+        if rc >= 0:
+            return _check(rc, where)
     dy, dys = _matrix(dy, dy_stride, tokens, hidden, datatype, where, "dy")
     z, zs = _matrix(z, z_stride, rows, hidden, datatype, where, "z")
     dz, dzs = _matrix(dz, dz_stride, rows, hidden, datatype, where, "dz")

@@ -475,6 +475,37 @@ def test_captured_sort_and_rows_replay():
             assert torch.equal(a[key].view(torch.uint8), b[key].view(torch.uint8)), (k, key)
 
 
+def test_device_pointers_and_streams_by_handle():
+    """The same calls with addresses, strides and a stream handle in the place of tensors."""
+    import torch
+    import rccl_amd as ra
+    r = Rows(50, 3, 100, "bf16", seed=6)
+    (_, x), (_, out), (_, y), (_, dz) = r.matrix(50), r.matrix(r.rows, 0.0), r.matrix(50, 0.0), r.matrix(r.rows, 0.0)
+    w, dw, ids = r.weights("f32"), torch.zeros(50, 3, device="cuda"), torch.from_numpy(r.ids.astype(np.int32)).cuda()
+    pos, off, cnt = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (150, 9, 8))
+
+    def run(at, stream, **strides):
+        ra.expert_sort(at(ids), ra.ncclInt32, 50, 3, 0, 8, 4, at(pos), None, at(off), at(cnt), None, stream=stream)
+        s = lambda *names: {n: v for n, v in strides.items() if n in names}  # noqa: E731
+        ra.expert_dispatch(at(x), at(out), r.rows, r.code, 50, 3, 100, at(pos), at(off), at(cnt), 8, stream=stream, **s("x_stride", "out_stride"))
+        ra.expert_combine(at(out), r.rows, at(w), ra.ncclFloat32, at(y), r.code, 50, 3, 100, at(pos), stream=stream, **s("z_stride", "y_stride"))
+        ra.expert_combine_backward(at(y), at(out), r.rows, at(w), ra.ncclFloat32, at(dz), at(dw), r.code, 50, 3, 100, at(pos), stream=stream, **s("dy_stride", "z_stride", "dz_stride"))
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (pos, off, cnt, out, y, dz, dw)]
+        for t in (pos, off, cnt, out, y, dz, dw):
+            t.zero_()
+        torch.cuda.synchronize()
+        return got
+
+    st = torch.cuda.Stream()
+    a = run(lambda t: t, None)
+    b = run(lambda t: t.data_ptr(), st.cuda_stream, x_stride=100, out_stride=100, z_stride=100, y_stride=100, dy_stride=100, dz_stride=100)
+    c = run(lambda t: t, st)
+    for p, q, v in zip(a, b, c):
+        assert torch.equal(p, q) and torch.equal(p, v)
+    assert np.array_equal(a[0].cpu().numpy(), r.position)
+
+
 def test_tensor_checks_of_the_python_mirror():
     import torch
     import rccl_amd as ra
