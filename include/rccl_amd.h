@@ -324,7 +324,7 @@ typedef struct {
  * An 8-bit state is rounded stochastically: a moving average with beta2 = 0.999 moves by less than half a step of an
  * 8-bit float in an update, and rounding to nearest would leave it where it is.  The random bits are a hash of (seed,
  * step, place of the tensor in the call, index of the element), so a step can be repeated exactly.  A sqrt(v) over zero is
- * never rounded to zero.  copyType is ignored where every copy is NULL.  tensors is host memory, read before the call
+ * never rounded to zero.  A moment that is not finite becomes NaN and does not count for its block's scale.  copyType is ignored where every copy is NULL.  tensors is host memory, read before the call
  * returns.  Tensors may not overlap one another. */
 ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntensors, ncclDataType_t paramType, ncclDataType_t gradType,
                           ncclDataType_t copyType, rcclAmdStateType_t stateType, const rcclAmdAdamWConfig_t* config,

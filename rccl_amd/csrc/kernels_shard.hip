@@ -99,10 +99,19 @@ static __device__ __forceinline__ uint32_t encode4(f32x4 x, uint32_t scale, cons
   c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[2], rnd[2], f, 2);
   return __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[3], rnd[3], f, 3);
 }
-static __device__ __forceinline__ uint32_t bitsMax(f32x4 x) {
+// Largest magnitude of a block, as a bit pattern.  What is not finite does not count: it becomes NaN, and the others of its
+// block keep their scale.  That costs a second pass, which only waves that hold such an element take.
+static __device__ __forceinline__ uint32_t largestOf8(f32x4 x) {
   uint32_t a = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) { const uint32_t b = __float_as_uint(x[i]) & 0x7FFFFFFFu; a = a > b ? a : b; }
+  a = maxOf8(a);
+  if (__any(a >= 0x7F800000u)) {
+    a = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const uint32_t b = __float_as_uint(x[i]) & 0x7FFFFFFFu; a = b > a && b < 0x7F800000u ? b : a; }
+    a = maxOf8(a);
+  }
   return a;
 }
 
@@ -171,7 +180,7 @@ template <typename P, typename G, bool MX> struct Row {
     storeCopy(at, whole, left);
     if constexpr (MX) {
       // (what does not exist is zero: its gradient and its moments were)
-      const uint32_t em = scaleOf(maxOf8(bitsMax(fm))), ev = scaleOf(maxOf8(bitsMax(r)));
+      const uint32_t em = scaleOf(largestOf8(fm)), ev = scaleOf(largestOf8(r));
       const float least = powerOf(ev) * 0x1p-9f;            // a second moment over zero stays over zero
       uint32_t rm[4], rv[4];                                // 16 random bits, and a half of the last of them
 #pragma unroll

@@ -22,6 +22,8 @@ static struct {
   __typeof__(&rcclAmdExpertDispatch) dispatch;
   __typeof__(&rcclAmdExpertCombine) combine;
   __typeof__(&rcclAmdExpertCombineBackward) combineBackward;
+  __typeof__(&rcclAmdSumSquaresBytes) sumSquaresBytes;
+  __typeof__(&rcclAmdExpertSortBytes) sortBytes;
 } fn;
 
 /* A call that is being put together: `ok` falls to 0 with the first argument that is not plain. */
@@ -255,15 +257,35 @@ static PyObject* mAdamW(PyObject* self, PyObject* const* a, Py_ssize_t nargs) {
   return done(&c, rc);
 }
 
+/* The sizes of workspaces: the bytes, or -1 where the arguments are not plain or are refused. */
+static PyObject* mExpertSortBytes(PyObject* self, PyObject* const* a, Py_ssize_t nargs) {
+  NEED(3);
+  Call c = {fn.sortBytes != NULL, 0};
+  size_t bytes = 0;
+  const size_t tokens = size(&c, a[0]);
+  const int topk = small(&c, a[1]), n = small(&c, a[2]);
+  if (c.ok && fn.sortBytes(tokens, topk, n, &bytes) != ncclSuccess) c.ok = 0;
+  return PyLong_FromSsize_t(c.ok ? (Py_ssize_t)bytes : -1);
+}
+static PyObject* mSumSquaresBytes(PyObject* self, PyObject* const* a, Py_ssize_t nargs) {
+  NEED(1);
+  Call c = {fn.sumSquaresBytes != NULL, 0};
+  size_t bytes = 0;
+  const int n = small(&c, a[0]);
+  if (c.ok && fn.sumSquaresBytes(n, &bytes) != ncclSuccess) c.ok = 0;
+  return PyLong_FromSsize_t(c.ok ? (Py_ssize_t)bytes : -1);
+}
+
 /* bind(element types by code, current device, current stream of a device, addresses of the library's functions) */
 static PyObject* mBind(PyObject* self, PyObject* args) {
   PyObject *t, *d, *s, *f;
   if (!PyArg_ParseTuple(args, "O!OOO!", &PyDict_Type, &t, &d, &s, &PyTuple_Type, &f)) return NULL;
-  void* p[6];
-  if (PyTuple_GET_SIZE(f) != 6) { PyErr_SetString(PyExc_TypeError, "six functions are needed"); return NULL; }
-  for (int i = 0; i < 6; i++) { p[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(f, i)); if (!p[i]) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "a null function"); return NULL; } }
+  void* p[8];
+  if (PyTuple_GET_SIZE(f) != 8) { PyErr_SetString(PyExc_TypeError, "eight functions are needed"); return NULL; }
+  for (int i = 0; i < 8; i++) { p[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(f, i)); if (!p[i]) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "a null function"); return NULL; } }
   fn.adamw = (__typeof__(fn.adamw))p[0]; fn.sumSquares = (__typeof__(fn.sumSquares))p[1]; fn.sort = (__typeof__(fn.sort))p[2];
   fn.dispatch = (__typeof__(fn.dispatch))p[3]; fn.combine = (__typeof__(fn.combine))p[4]; fn.combineBackward = (__typeof__(fn.combineBackward))p[5];
+  fn.sumSquaresBytes = (__typeof__(fn.sumSquaresBytes))p[6]; fn.sortBytes = (__typeof__(fn.sortBytes))p[7];
   for (int i = 0; i < ncclNumTypes; i++) {
     PyObject* key = PyLong_FromLong(i);
     PyObject* v = key ? PyDict_GetItem(t, key) : NULL;
@@ -284,6 +306,8 @@ static PyMethodDef methods[] = {
   {"expert_combine_backward", (PyCFunction)(void (*)(void))mExpertCombineBackward, METH_FASTCALL, NULL},
   {"sum_squares", (PyCFunction)(void (*)(void))mSumSquares, METH_FASTCALL, NULL},
   {"adamw", (PyCFunction)(void (*)(void))mAdamW, METH_FASTCALL, NULL},
+  {"expert_sort_bytes", (PyCFunction)(void (*)(void))mExpertSortBytes, METH_FASTCALL, NULL},
+  {"sum_squares_bytes", (PyCFunction)(void (*)(void))mSumSquaresBytes, METH_FASTCALL, NULL},
   {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mirror", "Plain calls of the local operators (see nccl.py).", -1, methods, NULL, NULL, NULL, NULL};
 

@@ -409,7 +409,8 @@ def _bind():
         _torch()
     L = lib()
     module.bind(_TORCH, _current_device, _current_stream, tuple(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in (
-        "rcclAmdAdamW", "rcclAmdSumSquares", "rcclAmdExpertSort", "rcclAmdExpertDispatch", "rcclAmdExpertCombine", "rcclAmdExpertCombineBackward")))
+        "rcclAmdAdamW", "rcclAmdSumSquares", "rcclAmdExpertSort", "rcclAmdExpertDispatch", "rcclAmdExpertCombine", "rcclAmdExpertCombineBackward",
+        "rcclAmdSumSquaresBytes", "rcclAmdExpertSortBytes")))
     _mirror = module
     return module
 
@@ -536,6 +537,8 @@ def adamw(tensors, param_type, grad_type, copy_type=-1, state_type=rcclAmdStateF
 
 def sum_squares_bytes(n):
     """rcclAmdSumSquaresBytes: bytes of workspace for `n` tensors."""
+    if _mirror and (nbytes := _mirror.sum_squares_bytes(n)) >= 0:
+        return nbytes
     v = ctypes.c_size_t()
     _check(lib().rcclAmdSumSquaresBytes(n, ctypes.byref(v)), "rcclAmdSumSquaresBytes")
     return v.value
@@ -568,6 +571,8 @@ def expert_rows(tokens, topk, n_experts, row_align=1):
 
 def expert_sort_bytes(tokens, topk, n_experts):
     """rcclAmdExpertSortBytes: bytes of workspace of expert_sort."""
+    if _mirror and (nbytes := _mirror.expert_sort_bytes(tokens, topk, n_experts)) >= 0:
+        return nbytes
     v = ctypes.c_size_t()
     _check(lib().rcclAmdExpertSortBytes(tokens, topk, n_experts, ctypes.byref(v)), "rcclAmdExpertSortBytes")
     return v.value

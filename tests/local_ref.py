@@ -42,10 +42,11 @@ def hash32(seed, step, ordinal, index):
 
 
 def mx_scale(x):
-    """The scale exponent (byte) of each block of 32: the smallest power of two with which all magnitudes are at most 448."""
+    """The scale exponent (byte) of each block of 32: the smallest power of two with which all finite magnitudes are at most 448."""
     out = np.ones(-(-x.size // 32), dtype=np.int64)
     for b in range(out.size):
-        most = float(np.max(np.abs(x[32 * b:32 * b + 32])))
+        block = np.abs(x[32 * b:32 * b + 32])
+        most = float(np.max(block[np.isfinite(block)], initial=0.0))
         while out[b] < 247 and most > 448.0 * 2.0 ** (int(out[b]) - 127):
             out[b] += 1
     return out.astype(np.uint8)
@@ -60,7 +61,8 @@ def mx_decode(code, scale):
 def mx_encode(x, rnd16, keep_positive):
     """(codes, scales) of fp32 values.  A value between two neighbours of the grid goes to the upper one where its distance
     from the lower one, in 2^20ths of their distance (cut to a whole number), and the 20 random bits together reach 2^20."""
-    scale = mx_scale(x)
+    scale, fine = mx_scale(x), np.isfinite(x)
+    x = np.where(fine, x, np.float32(0))
     y = np.abs(x.astype(np.float64)) / np.repeat(2.0 ** (scale.astype(np.float64) - 127), 32)[:x.size]
     # a value below 2^-6 passes through fp32 in the binade above (its 24 bits reach down to 2^-29)
     y = np.where(y < 2.0 ** -6, (y.astype(np.float32) + np.float32(2.0 ** -6)).astype(np.float64) - 2.0 ** -6, y)
@@ -70,7 +72,7 @@ def mx_encode(x, rnd16, keep_positive):
     code = low + (part + (rnd16.astype(np.int64) << 4 | 8) >= 2 ** 20)
     if keep_positive:
         code = np.where((x > 0) & (code == 0), 1, code)
-    return (code | np.where(np.signbit(x), 0x80, 0)).astype(np.uint8), scale
+    return np.where(fine, code | np.where(np.signbit(x), 0x80, 0), 0x7F).astype(np.uint8), scale
 
 
 # ------------------------------------------------------------------ AdamW

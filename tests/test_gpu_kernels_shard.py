@@ -296,20 +296,22 @@ def test_8_bit_rounding_is_unbiased():
 
 
 def test_8_bit_non_finite_gradients():
-    """An element whose moment is not finite becomes NaN; the scale of its block still has a value, other blocks are untouched by it."""
-    case = Case([256], "f32", "f32", None, mx=True, seed=22, scale=1e-4)
-    case.cut(case.grad, 0)[40] = float("inf")
-    case.cut(case.grad, 0)[200] = float("nan")
+    """An element whose moment is not finite becomes NaN; the others of its block are rounded as if it were not there."""
+    case = Case([256, 40], "f32", "f32", None, mx=True, seed=22, scale=1e-4)
+    for i, k, v in ((0, 40, "inf"), (0, 200, "nan"), (0, 201, "-inf"), (1, 39, "nan")):
+        case.cut(case.grad, i)[k] = float(v)
+    case.cut(case.grad, 0)[96:128] = float("inf")               # a block with nothing finite
     before = case.snapshot()
     case.run(seed=1)
-    m, v = _np(case.cut(case.m, 0)), _np(case.cut(case.v, 0))
-    assert (m[40] & 0x7F) == 0x7F and (m[200] & 0x7F) == 0x7F and (v[40] & 0x7F) == 0x7F and (v[200] & 0x7F) == 0x7F
-    fine = [b for b in range(8) if b not in (40 // 32, 200 // 32)]
-    case.cut(case.grad, 0)[40] = 0
-    case.cut(case.grad, 0)[200] = 0
-    want = _mx_expect(case, [case.grad.clone() if b is case.grad else o for b, o in zip(case.bufs, before)], 1.0, 1)[0]
-    for b in fine:
-        assert np.array_equal(m[32 * b:32 * b + 32], want[1][0][32 * b:32 * b + 32]) and _np(case.cut_scale(case.ms, 0))[b] == want[1][1][b]
+    with np.errstate(all="ignore"):
+        want = _mx_expect(case, before, 1.0, 1)
+    for i, (_, (cm, sm), (cv, sv)) in enumerate(want):
+        assert np.array_equal(_np(case.cut_scale(case.ms, i)), sm) and np.array_equal(_np(case.cut_scale(case.vs, i)), sv)
+        for buf, code in ((case.m, cm), (case.v, cv)):
+            got, bad = _np(case.cut(buf, i)), (code & 0x7F) == 0x7F
+            assert bad.sum() == (35 if i == 0 else 1) and np.all((got[bad] & 0x7F) == 0x7F)
+            assert np.array_equal(got[~bad], code[~bad])
+    assert np.isfinite(_np(case.cut(case.param, 0))).sum() == 256 - 35
 
 
 def test_8_bit_states_past_32_bits_of_elements():

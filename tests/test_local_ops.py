@@ -104,3 +104,17 @@ def test_rows_without_work():
     ra.expert_dispatch(None, None, 0, ra.ncclFloat32, 0, 1, 8, None, stream=0)
     ra.expert_combine(None, 0, None, -1, None, ra.ncclFloat32, 0, 1, 8, None, stream=0)
     ra.expert_combine_backward(None, None, 0, None, ra.ncclFloat32, None, None, ra.ncclFloat32, 0, 1, 8, None, stream=0)
+
+
+def test_the_mirror_module_leaves_what_is_not_plain():
+    """Arguments that it does not take are answered with -1 (the long way then says what is wrong), wrong numbers of them with
+    a TypeError; nothing is called."""
+    from rccl_amd import _mirror as m
+    for name, n in (("expert_sort", 13), ("expert_dispatch", 12), ("expert_combine", 11), ("expert_combine_backward", 16), ("sum_squares", 7), ("adamw", 18), ("expert_sort_bytes", 3), ("sum_squares_bytes", 1)):
+        for junk in (None, "x", object(), -1, 2 ** 70, 1.5):
+            assert getattr(m, name)(*[junk] * n) == -1, (name, junk)
+        with pytest.raises(TypeError):
+            getattr(m, name)()
+    for args in ((), ({}, None, None, ()), ({}, None, None, (1,) * 7), ({}, None, None, ("x",) * 8), ({}, None, None, (0,) * 8), ([], None, None, (1,) * 8)):
+        with pytest.raises((TypeError, ValueError)):
+            m.bind(*args)
