@@ -165,7 +165,7 @@ __global__ __launch_bounds__(RA_SORT_THREADS) void raLocalKernelSort(RaSortArgs 
 }
 
 hipError_t raLaunchSort(const RaSortArgs& a, hipStream_t s) {
-  const uint32_t rounds = raSortRounds(a.slots);
+  const uint32_t rounds = raSortRounds(a.slots, a.nExperts);
   if (a.tiles > 1) hipLaunchKernelGGL(raLocalKernelSortCount, dim3(a.tiles), dim3(RA_SORT_THREADS), a.nExperts * sizeof(int), s, a, RA_SORT_THREADS * rounds);
   if (a.scanned) hipLaunchKernelGGL(raLocalKernelSortScan, dim3((a.nExperts + 15) / 16), dim3(RA_SORT_THREADS), 0, s, a);
   switch (rounds) {

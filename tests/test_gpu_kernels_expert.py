@@ -70,6 +70,14 @@ def test_sort_at_the_limits(tokens, topk, n):
         assert np.array_equal(a, b)
 
 
+@pytest.mark.parametrize("tokens,topk,n", [(65536, 8, 16), (65537, 8, 17), (65536, 8, 128), (65537, 8, 128), (131073, 2, 1024), (300001, 8, 4), (300001, 8, 300)])
+def test_sort_at_tile_sizes(tokens, topk, n):
+    """Tiles of each size, with the counts of all tiles added up by every tile or by a launch in between, at both sides of the limit."""
+    ids = _ids(np.random.default_rng(tokens + n), tokens, topk, n, "padded")
+    for a, b in zip(_run_sort(ids, 0, n, 8, True), ref.expert_sort(ids, 0, n, 8)):
+        assert np.array_equal(a, b)
+
+
 def test_sort_of_ids_that_are_far_out():
     """Ids outside every range, the extremes of int64 among them, are dropped."""
     ids = np.array([[-2 ** 63, 2 ** 63 - 1], [2 ** 32, 2 ** 32 + 5], [5, -1], [6, 4], [7, 5]], dtype=np.int64)
