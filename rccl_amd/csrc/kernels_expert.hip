@@ -166,15 +166,16 @@ __global__ __launch_bounds__(RA_SORT_THREADS) void raLocalKernelSort(RaSortArgs 
 
 hipError_t raLaunchSort(const RaSortArgs& a, hipStream_t s) {
   const uint32_t rounds = raSortRounds(a.slots, a.nExperts);
-  if (a.tiles > 1) hipLaunchKernelGGL(raLocalKernelSortCount, dim3(a.tiles), dim3(RA_SORT_THREADS), a.nExperts * sizeof(int), s, a, RA_SORT_THREADS * rounds);
-  if (a.scanned) hipLaunchKernelGGL(raLocalKernelSortScan, dim3((a.nExperts + 15) / 16), dim3(RA_SORT_THREADS), 0, s, a);
+  hipError_t e = hipSuccess;
+  if (a.tiles > 1) e = raLaunch(raLocalKernelSortCount, a.tiles, RA_SORT_THREADS, a.nExperts * sizeof(int), s, a, RA_SORT_THREADS * rounds);
+  if (a.scanned && e == hipSuccess) e = raLaunch(raLocalKernelSortScan, (a.nExperts + 15) / 16, RA_SORT_THREADS, 0, s, a);
+  if (e != hipSuccess) return e;
   switch (rounds) {
-    case 1: hipLaunchKernelGGL((raLocalKernelSort<1>), dim3(a.tiles), dim3(RA_SORT_THREADS), sortLds(a.nExperts), s, a); break;
-    case 2: hipLaunchKernelGGL((raLocalKernelSort<2>), dim3(a.tiles), dim3(RA_SORT_THREADS), sortLds(a.nExperts), s, a); break;
-    case 4: hipLaunchKernelGGL((raLocalKernelSort<4>), dim3(a.tiles), dim3(RA_SORT_THREADS), sortLds(a.nExperts), s, a); break;
-    default: hipLaunchKernelGGL((raLocalKernelSort<8>), dim3(a.tiles), dim3(RA_SORT_THREADS), sortLds(a.nExperts), s, a); break;
+    case 1: return raLaunch(raLocalKernelSort<1>, a.tiles, RA_SORT_THREADS, sortLds(a.nExperts), s, a);
+    case 2: return raLaunch(raLocalKernelSort<2>, a.tiles, RA_SORT_THREADS, sortLds(a.nExperts), s, a);
+    case 4: return raLaunch(raLocalKernelSort<4>, a.tiles, RA_SORT_THREADS, sortLds(a.nExperts), s, a);
+    default: return raLaunch(raLocalKernelSort<8>, a.tiles, RA_SORT_THREADS, sortLds(a.nExperts), s, a);
   }
-  return hipGetLastError();
 }
 
 // ------------------------------------------------------------------ rows
@@ -391,8 +392,8 @@ static __device__ __forceinline__ void combineAt(const RaRowsArgs& a, T* y, uint
 #pragma unroll
   for (int u = 0; u < U; u++) if (WHOLE || at + u * 64 * N < end) storeWhole<true>(y + at + u * 64 * N, fromFloats<T>(sum[u]));
 }
-// The same for one element of each lane.
-template <typename T> static __device__ __forceinline__ void combineElement(const RaRowsArgs& a, T* y, uint32_t at, uint64_t slots, int32_t pos, float w) {
+// The same for one element of each lane that has one.  All lanes run through it: what a slot has lies in the lane of its number.
+template <typename T> static __device__ __forceinline__ void combineElement(const RaRowsArgs& a, T* y, uint32_t at, bool go, uint64_t slots, int32_t pos, float w) {
   constexpr int F = 8;
   float sum = 0.f;
   while (slots) {
@@ -404,12 +405,13 @@ template <typename T> static __device__ __forceinline__ void combineElement(cons
       const int k = __builtin_ctzll(slots);
       slots &= slots - 1;
       wk[f] = laneFloat(w, k);
-      z[f] = (float)((const T*)a.in)[(size_t)laneInt(pos, k) * a.inStride + at];
+      const size_t row = (size_t)laneInt(pos, k) * a.inStride;
+      if (go) z[f] = (float)((const T*)a.in)[row + at];
     }
 #pragma unroll
     for (int f = 0; f < F; f++) sum = __builtin_fmaf(wk[f], z[f], sum);      // (a slot that is not there adds 0 * 0)
   }
-  y[at] = (T)sum;
+  if (go) y[at] = (T)sum;
 }
 template <typename T>
 __global__ __launch_bounds__(RA_COMBINE_THREADS) void raLocalKernelCombine(RaRowsArgs a, uint32_t parts, uint32_t partElems) {
@@ -433,7 +435,7 @@ __global__ __launch_bounds__(RA_COMBINE_THREADS) void raLocalKernelCombine(RaRow
     if (partElems == 64 * N) combineAt<T, 1, false>(a, y, at, end, slots, pos, w);
     else if (c.head + run + U * 64 * N <= end) combineAt<T, U, true>(a, y, at, end, slots, pos, w);
     else combineAt<T, U, false>(a, y, at, end, slots, pos, w);
-    if (run == 0 && lane < c.single) combineElement(a, y, elementOf(c.head, a.hidden, c.single, lane), slots, pos, w);
+    if (run == 0 && c.single) combineElement(a, y, elementOf(c.head, a.hidden, c.single, lane), lane < c.single, slots, pos, w);
   }
 }
 
@@ -612,15 +614,13 @@ template <typename T> static uint32_t narrowShift(const RaRowsArgs& a) {
 }
 template <typename T, int S>
 static hipError_t launchDispatch(const RaRowsArgs& a, uint32_t groups, int threads, uint32_t parts, uint32_t partElems, hipStream_t s) {
-  if (groups + padGroups(a)) hipLaunchKernelGGL((raLocalKernelDispatch<T, S>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups, parts, partElems);
-  return hipGetLastError();
+  return raLaunch(raLocalKernelDispatch<T, S>, groups + padGroups(a), threads, 0, s, a, groups, parts, partElems);
 }
 template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_t s) {
   const uint32_t shift = narrowShift<T>(a);
   if (shift < 6) {
     const uint32_t groups = groupsOf(((uint64_t)a.tokens * a.topk + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS);
-    if (groups + padGroups(a)) hipLaunchKernelGGL(raLocalKernelDispatchNarrow<T>, dim3(groups + padGroups(a)), dim3(RA_NARROW_THREADS), 0, s, a, groups, shift);
-    return hipGetLastError();
+    return raLaunch(raLocalKernelDispatchNarrow<T>, groups + padGroups(a), RA_NARROW_THREADS, 0, s, a, groups, shift);
   }
   const uint64_t slots = (uint64_t)a.tokens * a.topk, step = 64 * Pack<T>::N;
   const int threads = slotThreads(a.topk);
@@ -639,36 +639,27 @@ template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_
 template <typename T> static hipError_t combine(const RaRowsArgs& a, hipStream_t s) {
   const uint32_t shift = narrowShift<T>(a);
   if (shift < 6) {
-    hipLaunchKernelGGL(raLocalKernelCombineNarrow<T>, dim3(groupsOf((a.tokens + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS)), dim3(RA_NARROW_THREADS), 0, s, a, shift);
-    return hipGetLastError();
+    return raLaunch(raLocalKernelCombineNarrow<T>, groupsOf((a.tokens + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS), RA_NARROW_THREADS, 0, s, a, shift);
   }
   const uint64_t step = 64 * Pack<T>::N;
   // four runs of 64 packs for each wave, or one where that leaves fewer than 4096 waves
   const size_t partElems = a.tokens * ((a.hidden + 4 * step - 1) / (4 * step)) < 4096 ? step : 4 * step;
   const uint64_t parts = (a.hidden + partElems - 1) / partElems;
-  hipLaunchKernelGGL(raLocalKernelCombine<T>, dim3(groupsOf(a.tokens * parts, RA_COMBINE_THREADS)), dim3(RA_COMBINE_THREADS), 0, s, a, (uint32_t)parts, (uint32_t)partElems);
-  return hipGetLastError();
+  return raLaunch(raLocalKernelCombine<T>, groupsOf(a.tokens * parts, RA_COMBINE_THREADS), RA_COMBINE_THREADS, 0, s, a, (uint32_t)parts, (uint32_t)partElems);
 }
 template <typename T> static hipError_t combineBackward(const RaRowsArgs& a, hipStream_t s) {
   const uint32_t shift = narrowShift<T>(a);
   if (shift < 6) {
     const uint32_t groups = groupsOf(((uint64_t)a.tokens * a.topk + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS);
-    hipLaunchKernelGGL(raLocalKernelCombineBackwardNarrow<T>, dim3(groups + padGroups(a)), dim3(RA_NARROW_THREADS), 0, s, a, groups, shift);
-    return hipGetLastError();
+    return raLaunch(raLocalKernelCombineBackwardNarrow<T>, groups + padGroups(a), RA_NARROW_THREADS, 0, s, a, groups, shift);
   }
   const int threads = slotThreads(a.topk);
   const uint64_t slots = (uint64_t)a.tokens * a.topk, runs = (a.hidden + 64 * Pack<T>::N - 1) / (64 * Pack<T>::N);
-  if (runs <= 1 && slots >= 4096 * 4) {
-    const uint32_t groups = groupsOf((slots + 3) / 4, threads);
-    hipLaunchKernelGGL((raLocalKernelCombineBackward<T, 4>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups);
-  } else if (runs <= 2 && slots >= 4096 * 2) {
-    const uint32_t groups = groupsOf((slots + 1) / 2, threads);
-    hipLaunchKernelGGL((raLocalKernelCombineBackward<T, 2>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups);
-  } else {
-    const uint32_t groups = groupsOf(slots, threads);
-    hipLaunchKernelGGL((raLocalKernelCombineBackward<T, 1>), dim3(groups + padGroups(a)), dim3(threads), 0, s, a, groups);
-  }
-  return hipGetLastError();
+  const int each = runs <= 1 && slots >= 4096 * 4 ? 4 : runs <= 2 && slots >= 4096 * 2 ? 2 : 1;
+  const uint32_t groups = groupsOf((slots + each - 1) / each, threads);
+  return each == 4 ? raLaunch(raLocalKernelCombineBackward<T, 4>, groups + padGroups(a), threads, 0, s, a, groups)
+       : each == 2 ? raLaunch(raLocalKernelCombineBackward<T, 2>, groups + padGroups(a), threads, 0, s, a, groups)
+                   : raLaunch(raLocalKernelCombineBackward<T, 1>, groups + padGroups(a), threads, 0, s, a, groups);
 }
 #define RA_BY_TYPE(fn)                                    \
   switch (type) {                                         \

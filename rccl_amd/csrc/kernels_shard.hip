@@ -297,9 +297,7 @@ __global__ __launch_bounds__(RA_ADAMW_THREADS) __attribute__((amdgpu_waves_per_e
 
 template <typename P, typename G>
 static hipError_t adamW(const RaAdamWArgs& a, bool mx, uint32_t grid, hipStream_t s) {
-  if (mx) hipLaunchKernelGGL((raLocalKernelAdamW<P, G, true>), dim3(grid), dim3(RA_ADAMW_THREADS), 0, s, a);
-  else hipLaunchKernelGGL((raLocalKernelAdamW<P, G, false>), dim3(grid), dim3(RA_ADAMW_THREADS), 0, s, a);
-  return hipGetLastError();
+  return mx ? raLaunch(raLocalKernelAdamW<P, G, true>, grid, RA_ADAMW_THREADS, 0, s, a) : raLaunch(raLocalKernelAdamW<P, G, false>, grid, RA_ADAMW_THREADS, 0, s, a);
 }
 template <typename P>
 static hipError_t adamWGrad(const RaAdamWArgs& a, int gradType, bool mx, uint32_t grid, hipStream_t s) {
@@ -380,14 +378,12 @@ __global__ __launch_bounds__(1024) void raLocalKernelSumSqJoin(const double* __r
 
 hipError_t raLaunchSumSq(const RaSumSqArgs& a, int type, uint32_t grid, hipStream_t s) {
   switch (type) {
-    case ncclFloat32: hipLaunchKernelGGL((raLocalKernelSumSq<float>), dim3(grid), dim3(RA_SUMSQ_THREADS), 0, s, a); break;
-    case ncclBfloat16: hipLaunchKernelGGL((raLocalKernelSumSq<__bf16>), dim3(grid), dim3(RA_SUMSQ_THREADS), 0, s, a); break;
-    case ncclFloat16: hipLaunchKernelGGL((raLocalKernelSumSq<_Float16>), dim3(grid), dim3(RA_SUMSQ_THREADS), 0, s, a); break;
+    case ncclFloat32: return raLaunch(raLocalKernelSumSq<float>, grid, RA_SUMSQ_THREADS, 0, s, a);
+    case ncclBfloat16: return raLaunch(raLocalKernelSumSq<__bf16>, grid, RA_SUMSQ_THREADS, 0, s, a);
+    case ncclFloat16: return raLaunch(raLocalKernelSumSq<_Float16>, grid, RA_SUMSQ_THREADS, 0, s, a);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 hipError_t raLaunchSumSqJoin(const double* partial, uint32_t n, double* out, int accumulate, hipStream_t s) {
-  hipLaunchKernelGGL(raLocalKernelSumSqJoin, dim3(1), dim3(1024), 0, s, partial, n, out, accumulate);
-  return hipGetLastError();
+  return raLaunch(raLocalKernelSumSqJoin, 1, 1024, 0, s, partial, n, out, accumulate);
 }

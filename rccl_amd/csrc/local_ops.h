@@ -6,6 +6,15 @@
 
 #include "rccl_amd.h"
 
+// Launches a kernel and returns what that launch says.  (The error that hipGetLastError gives may be an older one of the
+// caller's program, which is not this library's to report or to clear.)
+template <typename T> struct RaSame { typedef T type; };
+template <typename... A>
+static inline hipError_t raLaunch(void (*kernel)(A...), uint32_t grid, int block, size_t lds, hipStream_t s, const typename RaSame<A>::type&... args) {
+  void* p[] = {(void*)&args...};
+  return hipLaunchKernel((const void*)kernel, dim3(grid), dim3((unsigned)block), p, lds, s);
+}
+
 // ------------------------------------------------------------------ AdamW, sum of squares
 // Everything a launch needs travels in its arguments (at most 4 KiB): no table in device memory, nothing to allocate or to
 // keep alive, and a captured launch stays valid.  In the general form a tensor takes `stride` words: the pointers the launch
