@@ -278,9 +278,9 @@ ncclResult_t rcclAmdNoAllocAsyncError(int device, ncclResult_t* asyncError);
 /* ---- local operators of a sharded training step ------------------------------------------------
  * What a rank computes between a reduce-scatter and an all-gather: the optimizer step of its shard, and the sorting,
  * dispatching and combining of token rows for the experts it holds.  Like rcclAmdReduceCopy they run on the current
- * device, are enqueued on `stream`, allocate nothing, keep nothing from one call for the next, never wait for the GPU, and
- * may be captured into a graph (a captured call keeps the pointers and host values that it was captured with).  Buffers
- * are device memory of the current device; workspaces belong to the caller, must be 16-byte aligned and may not be shared
+ * device, are enqueued on `stream` (a stream of that device), allocate nothing, keep nothing from one call for the next,
+ * never wait for the GPU, and may be captured into a graph (a captured call keeps the pointers and host values that it was
+ * captured with).  Buffers are device memory of the current device; workspaces belong to the caller, must be 16-byte aligned and may not be shared
  * by calls that can run at the same time.  Floating types: ncclFloat32, ncclBfloat16, ncclFloat16; every pointer has the
  * alignment of its element type, no more is asked.  Outputs may not overlap inputs unless a call says so.  Results do not
  * depend on the order in which the GPU runs things: the same call on the same data gives the same bits. */
@@ -324,8 +324,9 @@ typedef struct {
  * An 8-bit state is rounded stochastically: a moving average with beta2 = 0.999 moves by less than half a step of an
  * 8-bit float in an update, and rounding to nearest would leave it where it is.  The random bits are a hash of (seed,
  * step, place of the tensor in the call, index of the element), so a step can be repeated exactly.  A sqrt(v) over zero is
- * never rounded to zero.  A moment that is not finite becomes NaN and does not count for its block's scale.  copyType is ignored where every copy is NULL.  tensors is host memory, read before the call
- * returns.  Tensors may not overlap one another. */
+ * never rounded to zero.  A moment that is not finite becomes NaN and does not count for its block's scale.
+ * eps is 0 or a normal fp32 number.  copyType is ignored where every copy is NULL.  tensors is host memory, read before the
+ * call returns.  Tensors may not overlap one another. */
 ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntensors, ncclDataType_t paramType, ncclDataType_t gradType,
                           ncclDataType_t copyType, rcclAmdStateType_t stateType, const rcclAmdAdamWConfig_t* config,
                           hipStream_t stream);

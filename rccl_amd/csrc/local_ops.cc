@@ -1,4 +1,5 @@
 // The exported local operators of a sharded training step: argument checks, how work is cut, launches.
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -20,6 +21,14 @@
     }                                                                                \
   } while (0)
 
+// Kernels run on the current device; a stream of another one would take them, and buffers they may not reach, there.
+static ncclResult_t checkStream(const char* fn, hipStream_t stream) {
+  int own = 0, current = 0;
+  if ((uintptr_t)stream <= (uintptr_t)hipStreamPerThread) return ncclSuccess;      // the default streams are the current device's
+  if (hipStreamGetDevice(stream, &own) != hipSuccess || hipGetDevice(&current) != hipSuccess) RA_REFUSE("%s: the stream has no device", fn);
+  if (own != current) RA_REFUSE("%s: the stream belongs to device %d, the current device is %d", fn, own, current);
+  return ncclSuccess;
+}
 static bool isFloat(int t) { return t == ncclFloat32 || t == ncclBfloat16 || t == ncclFloat16; }
 static bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 static const uint64_t kMaxElements = 1ull << 40;      // of one call: byte offsets and chunk numbers stay far from overflow
@@ -71,6 +80,7 @@ RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntenso
   const rcclAmdAdamWConfig_t& c = *config;
   if (!isfinite(c.lr) || !isfinite(c.weightDecay) || !isfinite(c.gradScale) || !isfinite(c.eps) || c.eps < 0.0 || c.gradScale < 0.0)
     RA_REFUSE("%s: lr, weightDecay, gradScale and eps must be finite, gradScale and eps not negative", fn);
+  if (c.eps > 0.0 && c.eps < FLT_MIN) RA_REFUSE("%s: eps %g is below the smallest normal fp32 number", fn, c.eps);
   if (!(c.beta1 >= 0.0 && c.beta1 < 1.0 && c.beta2 >= 0.0 && c.beta2 < 1.0)) RA_REFUSE("%s: beta1 = %g, beta2 = %g outside 0 <= beta < 1", fn, c.beta1, c.beta2);
   if (!c.stepPtr && c.step < 1) RA_REFUSE("%s: step %lld: the first step is 1", fn, (long long)c.step);
   if (c.sumSq && !(c.maxNorm >= 0.0)) RA_REFUSE("%s: maxNorm %g with sumSq", fn, c.maxNorm);
@@ -89,6 +99,7 @@ RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntenso
     copies = copies || t.copy;
   }
   if (copies && !isFloat(copyType)) RA_REFUSE("%s: copy type %d is not float32, bfloat16 or float16", fn, (int)copyType);
+  if (all) RA_CHECK(checkStream(fn, stream));
 
   RaAdamWArgs a;
   a.lr = c.lr; a.beta1 = c.beta1; a.beta2 = c.beta2; a.weightDecay = c.weightDecay; a.gradScale = c.gradScale; a.maxNorm = c.maxNorm;
@@ -156,6 +167,7 @@ RA_API ncclResult_t rcclAmdSumSquares(const void* const* tensors, const size_t* 
     if (counts[i] > kMaxElements || (all += counts[i]) > kMaxElements) RA_REFUSE("%s: tensor %d: %zu elements, or too many in all", fn, i, counts[i]);
     if (counts[i] && (!tensors[i] || !aligned(tensors[i], size))) RA_REFUSE("%s: tensor %d is null or not aligned to its element type", fn, i);
   }
+  RA_CHECK(checkStream(fn, stream));
   // Chunks: at most 4096 of equal size and one more for each tensor (and for each 2^31 elements of one, which is what an
   // entry of a launch holds), so the partial sums fit the workspace.
   const uint64_t unit = RA_SUMSQ_THREADS * 4 * 4, piece = 1ull << 31;
@@ -223,6 +235,7 @@ RA_API ncclResult_t rcclAmdExpertSort(const void* experts, ncclDataType_t expert
   if (!aligned(experts, raTypeSize(expertType)) || !aligned(position, 4) || !aligned(source, 4) || !aligned(offsets, 4) || !aligned(counts, 4) || !aligned(workspace, 16))
     RA_REFUSE("%s: misaligned buffer", fn);
   if (workspaceBytes < need || (need && !workspace)) RA_REFUSE("%s: workspace of %zu bytes, %zu needed", fn, workspaceBytes, need);
+  RA_CHECK(checkStream(fn, stream));
   RaSortArgs a;
   a.ids = experts; a.firstExpert = firstExpert; a.position = position; a.source = source; a.offsets = offsets; a.counts = counts;
   a.tileCounts = (int32_t*)workspace; a.slots = (uint32_t)slots; a.rows = (uint32_t)rows;
@@ -261,6 +274,7 @@ RA_API ncclResult_t rcclAmdExpertDispatch(const void* x, size_t xStride, void* o
   RA_CHECK(checkRows(fn, a, datatype, rows));
   if (rows && x == out) RA_REFUSE("%s: x and out are the same buffer", fn);
   if (rows == 0 || (tokens == 0 && !offsets)) return ncclSuccess;
+  RA_CHECK(checkStream(fn, stream));
   RA_LAUNCH(fn, raLaunchDispatch(a, datatype, stream));
   return ncclSuccess;
 }
@@ -276,6 +290,7 @@ RA_API ncclResult_t rcclAmdExpertCombine(const void* z, size_t zStride, size_t r
   RA_CHECK(checkRows(fn, a, datatype, tokens));
   if (tokens && rows && z == y) RA_REFUSE("%s: z and y are the same buffer", fn);
   if (tokens == 0) return ncclSuccess;
+  RA_CHECK(checkStream(fn, stream));
   RA_LAUNCH(fn, raLaunchCombine(a, datatype, stream));
   return ncclSuccess;
 }
@@ -294,6 +309,7 @@ RA_API ncclResult_t rcclAmdExpertCombineBackward(const void* dy, size_t dyStride
   if (rows && (dy == dz || dy == z || (z == dz && zStride != dzStride))) RA_REFUSE("%s: dy overlaps, or dz is z with another stride", fn);
   if (tokens && (dweights == weights)) RA_REFUSE("%s: weights and dweights are the same buffer", fn);
   if (tokens == 0 && (rows == 0 || !offsets)) return ncclSuccess;
+  RA_CHECK(checkStream(fn, stream));
   RA_LAUNCH(fn, raLaunchCombineBackward(a, datatype, stream));
   return ncclSuccess;
 }

@@ -121,7 +121,7 @@ static int64_t* table(Call* c, PyObject* x, Py_ssize_t columns, Py_buffer* b, Py
   *rows = 0;
   if (!c->ok || !PyObject_CheckBuffer(x) || PyObject_GetBuffer(x, b, PyBUF_C_CONTIGUOUS | PyBUF_FORMAT) != 0) { PyErr_Clear(); c->ok = 0; return NULL; }
   const char* f = b->format ? b->format : "B";
-  if (b->itemsize != 8 || f[1] != 0 || !strchr("lqLQ", f[0]) || b->ndim != (columns == 1 ? 1 : 2) || (columns > 1 && b->shape[1] != columns) || b->shape[0] > INT_MAX) { c->ok = 0; return NULL; }
+  if (b->itemsize != 8 || !f[0] || f[1] != 0 || !strchr("lqLQ", f[0]) || b->ndim != (columns == 1 ? 1 : 2) || (columns > 1 && b->shape[1] != columns) || b->shape[0] > INT_MAX) { c->ok = 0; return NULL; }
   *rows = b->shape[0];
   return (int64_t*)b->buf;
 }

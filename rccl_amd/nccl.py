@@ -499,22 +499,33 @@ def _host_table(x, columns, where):
     return face["data"][0], shape[0], a
 
 
-def adamw_tensor(param, grad, exp_avg, exp_avg_sq, count=None, exp_avg_scale=None, exp_avg_sq_scale=None, copy=None):
-    """One row of the table that adamw() takes, from contiguous tensors or device pointers (then with `count`)."""
-    tensors = [x for x in (param, grad, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, copy) if x is not None and not isinstance(x, int)]
+def adamw_tensor(param, grad, exp_avg, exp_avg_sq, count=None, exp_avg_scale=None, exp_avg_sq_scale=None, copy=None, *, param_type=None, grad_type=None,
+                 copy_type=None):
+    """One row of the table that adamw() takes, from contiguous tensors or device pointers (then with `count`).  Moments with
+    scales are bytes, those without are float32.  The row holds addresses, not types: with the types that adamw() will be
+    given, tensors of other ones are refused here."""
+    where = "adamw_tensor"
     if count is None:
         if isinstance(param, int):
-            _refuse("adamw_tensor", "a device pointer needs a count")
+            _refuse(where, "a device pointer needs a count")
         count = param.numel()
     blocks = -(-count // STATE_BLOCK)
-    if tensors and not _TORCH:
-        _torch()
-    for x in tensors:
-        need = blocks if x is exp_avg_scale or x is exp_avg_sq_scale else count
-        if x.get_device() != _current_device() or x.numel() < need or not x.is_contiguous():
-            _unfit(x, None, "adamw_tensor", "a tensor", f"{need} contiguous elements are")
-    at = lambda x: 0 if x is None else x if isinstance(x, int) else x.data_ptr()  # noqa: E731
-    return [at(param), at(grad), at(exp_avg), at(exp_avg_sq), at(exp_avg_scale), at(exp_avg_sq_scale), at(copy), count]
+    state = 1 if exp_avg_scale is not None or exp_avg_sq_scale is not None else 4
+    row = []
+    for name, x, datatype, size, need in (("param", param, param_type, None, count), ("grad", grad, grad_type, None, count), ("exp_avg", exp_avg, None, state, count),
+                                          ("exp_avg_sq", exp_avg_sq, None, state, count), ("exp_avg_scale", exp_avg_scale, None, 1, blocks),
+                                          ("exp_avg_sq_scale", exp_avg_sq_scale, None, 1, blocks), ("copy", copy, copy_type, None, count)):
+        if x is None or isinstance(x, int):
+            row.append(x or 0)
+            continue
+        if not _TORCH:
+            _torch()
+        if x.get_device() != _current_device() or x.numel() < need or not x.is_contiguous() or (datatype is not None and x.dtype is not _TORCH.get(datatype)):
+            _unfit(x, datatype, where, name, f"{need} contiguous elements are")
+        if size is not None and (x.element_size() != size or (size == 4 and x.dtype is not _TORCH[ncclFloat32])):
+            _refuse(where, f"{name} is {x.dtype}, {'float32' if size == 4 else 'bytes'} needed")
+        row.append(x.data_ptr())
+    return row + [count]
 
 
 def adamw(tensors, param_type, grad_type, copy_type=-1, state_type=rcclAmdStateF32, *, lr, beta1=0.9, beta2=0.999, eps=1e-8,

@@ -559,6 +559,39 @@ def test_on_another_stream():
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
 
+def test_element_types_of_a_row():
+    """Moments of the wrong size, or parameters that are not of the type adamw() will be given, would be read past their end."""
+    import torch
+    import rccl_amd as ra
+    f, h = torch.zeros(64, device="cuda"), torch.zeros(64, dtype=torch.bfloat16, device="cuda")
+    b, sc = torch.zeros(64, dtype=torch.uint8, device="cuda"), torch.zeros(2, dtype=torch.uint8, device="cuda")
+    t = dict(param_type=ra.ncclFloat32, grad_type=ra.ncclBfloat16, copy_type=ra.ncclFloat16)
+    assert ra.adamw_tensor(f, h, f, f, **t) == ra.adamw_tensor(f.data_ptr(), h, f, f, 64)
+    assert ra.adamw_tensor(f, h, b, b, exp_avg_scale=sc, exp_avg_sq_scale=sc, copy=h.half(), **t)[7] == 64
+    for call in (lambda: ra.adamw_tensor(f, f, b, f), lambda: ra.adamw_tensor(f, f, f, h), lambda: ra.adamw_tensor(f, f, f, f.int()),
+                 lambda: ra.adamw_tensor(f, f, f, f, exp_avg_scale=sc, exp_avg_sq_scale=sc), lambda: ra.adamw_tensor(f, f, b, b, exp_avg_scale=sc.int(), exp_avg_sq_scale=sc),
+                 lambda: ra.adamw_tensor(h, h, f, f, **t), lambda: ra.adamw_tensor(f, f, f, f, **t), lambda: ra.adamw_tensor(f, h, f, f, copy=f, **t)):
+        with pytest.raises(ra.NcclError) as e:
+            call()
+        assert e.value.code == ra.ncclInvalidArgument
+
+
+def test_an_older_error_is_not_reported_by_a_launch():
+    """A call reports what its own launches say; the error that another call of the program left stays with the program."""
+    import ctypes
+    import torch
+    hip = ctypes.CDLL(next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line))      # the one in use
+    a, b = (Case([1000], "f32", "f32", None, seed=5) for _ in range(2))
+    a.run()
+    torch.cuda.synchronize()
+    assert hip.hipSetDevice(1000) != 0                     # refused by the host, and remembered
+    b.run()
+    assert hip.hipGetLastError() != 0
+    torch.cuda.synchronize()
+    for x, y in zip(a.bufs, b.bufs):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
 def test_tensor_checks_of_the_python_mirror():
     """Tensors of another type, size or place are refused before an address is taken."""
     import torch

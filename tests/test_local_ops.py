@@ -39,6 +39,11 @@ def test_adamw_refusals(kw, text):
     _refused(lambda: _adamw(**kw), text)
 
 
+@pytest.mark.parametrize("eps", [1e-40, 2.0 ** -127, 5e-324])
+def test_adamw_refuses_an_eps_that_fp32_does_not_hold_as_a_normal_number(eps):
+    _refused(lambda: _adamw(eps=eps), "normal fp32")
+
+
 def test_adamw_without_work():
     _adamw(rows=np.zeros((0, 8)))
     _adamw(rows=[[0] * 8] * 200)                               # empty tensors need no buffers
