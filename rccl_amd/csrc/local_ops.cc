@@ -215,7 +215,7 @@ RA_API ncclResult_t rcclAmdExpertSortBytes(size_t tokens, int topk, int nExperts
   const char* fn = "rcclAmdExpertSortBytes";
   RA_CHECK(checkSlots(fn, tokens, topk));
   if (nExperts < 1 || nExperts > RA_SORT_MAX_EXPERTS || !workspaceBytes) RA_REFUSE("%s: %d experts, 1 .. %d supported, or a null argument", fn, nExperts, RA_SORT_MAX_EXPERTS);
-  const uint64_t tiles = raSortTiles((uint64_t)tokens * topk, nExperts);
+  const uint64_t tiles = raSortTiles((uint64_t)tokens * topk);
   *workspaceBytes = tiles > 1 ? (size_t)(tiles + 1) * nExperts * sizeof(int32_t) : 0;
   return ncclSuccess;
 }
@@ -239,7 +239,7 @@ RA_API ncclResult_t rcclAmdExpertSort(const void* experts, ncclDataType_t expert
   RaSortArgs a;
   a.ids = experts; a.firstExpert = firstExpert; a.position = position; a.source = source; a.offsets = offsets; a.counts = counts;
   a.tileCounts = (int32_t*)workspace; a.slots = (uint32_t)slots; a.rows = (uint32_t)rows;
-  a.tiles = slots ? (uint32_t)raSortTiles(slots, nExperts) : 1;
+  a.tiles = slots ? (uint32_t)raSortTiles(slots) : 1;
   a.nExperts = nExperts; a.rowAlign = rowAlign; a.idBytes = (int)raTypeSize(expertType);
   a.scanned = raSortScanned(a.tiles, nExperts);
   RA_LAUNCH(fn, raLaunchSort(a, stream));

@@ -81,26 +81,22 @@ struct RaSortArgs {
   int nExperts, rowAlign, idBytes;
   bool scanned;                      // raSortScanned
 };
-// The next power of two of the number of experts.
-static inline __host__ __device__ uint32_t raSortWidth(int nExperts) { return nExperts <= 1 ? 1 : 1u << (32 - __builtin_clz((unsigned)nExperts - 1)); }
-#define RA_SORT_COUNTS (16 * RA_SORT_THREADS)      // counts that every tile adds up by itself: 16 steps of its threads
 // Rounds of 64 slots a wave takes in one tile (a tile is RA_SORT_THREADS * rounds): one tile up to 4096 slots, which is one
-// launch; beyond that the smallest of 2 and 4 with which no launch in between is needed, otherwise by the number of slots.
-// In us, with 2, 4 and 8 rounds: 131072 slots of 256 experts 12.6, 13.0, 17.2; 524288 of 16 experts 8.8, 9.7, 13.1, of 128 experts
-// 19.1, 16.1, 18.3, of 384 experts 20.7, 19.1, 22.3; 4.2 million of 16 experts 85, 33, 33, of 128 experts 107, 72, 59.
-static inline uint32_t raSortRounds(uint64_t slots, int nExperts) {
-  if (slots <= 4 * RA_SORT_THREADS) return slots <= RA_SORT_THREADS ? 1 : slots <= 2 * RA_SORT_THREADS ? 2 : 4;
-  for (uint32_t r = 2; r <= 4; r *= 2)
-    if ((slots + RA_SORT_THREADS * r - 1) / (RA_SORT_THREADS * r) * raSortWidth(nExperts) <= RA_SORT_COUNTS) return r;
-  return slots <= 1u << 18 ? 2 : slots <= 1u << 21 ? 4 : 8;
+// launch; beyond that 2, and 4 for many tiles.  In us, with 2, 4 and 8 rounds: 131072 slots of 256 experts 11.0, 13.5, 18.7; 524288 of 128
+// experts 13.2, 14.6, 18.4; 1 million 16.6, 17.6, 21.7; 2 million of 64 experts 25.4, 23.0, 24.8; 4.2 million of 128 experts 46.6, 42.1, 45.3.
+static inline uint32_t raSortRounds(uint64_t slots) {
+  return slots <= 1024 ? 1 : slots <= 2048 ? 2 : slots <= 4096 ? 4 : slots <= 1u << 20 ? 2 : 4;
 }
-static inline uint64_t raSortTiles(uint64_t slots, int nExperts) {
-  const uint64_t tile = (uint64_t)RA_SORT_THREADS * raSortRounds(slots, nExperts);
+static inline uint64_t raSortTiles(uint64_t slots) {
+  const uint64_t tile = (uint64_t)RA_SORT_THREADS * raSortRounds(slots);
   return (slots + tile - 1) / tile;
 }
-// Every tile adds up the counts of all tiles by itself where they are few; otherwise a launch between the two does it once
-// (524288 slots of 384 experts: 30.2 us without it, 19.1 with it; of 128 experts 16.0 and 17.4).
-static inline bool raSortScanned(uint64_t tiles, int nExperts) { return tiles > 1 && tiles * raSortWidth(nExperts) > RA_SORT_COUNTS; }
+// The next power of two of the number of experts.
+static inline __host__ __device__ uint32_t raSortWidth(int nExperts) { return nExperts <= 1 ? 1 : 1u << (32 - __builtin_clz((unsigned)nExperts - 1)); }
+// Every tile adds up the counts of all tiles by itself where that is at most 8 steps of its threads; otherwise a launch between
+// the two does it once (524288 slots of 16 experts: 8.8 us without it, 10.9 with it; 131072 of 128 experts 9.8 and 10.5, of 256
+// experts 12.5 and 11.0).
+static inline bool raSortScanned(uint64_t tiles, int nExperts) { return tiles > 1 && tiles * raSortWidth(nExperts) > 8 * RA_SORT_THREADS; }
 hipError_t raLaunchSort(const RaSortArgs& a, hipStream_t s);
 
 #define RA_ROWS_MAX_TOPK 64

@@ -70,7 +70,7 @@ def test_sort_at_the_limits(tokens, topk, n):
         assert np.array_equal(a, b)
 
 
-@pytest.mark.parametrize("tokens,topk,n", [(65536, 8, 16), (65537, 8, 17), (65536, 8, 128), (65537, 8, 128), (131073, 2, 1024), (300001, 8, 4), (300001, 8, 300)])
+@pytest.mark.parametrize("tokens,topk,n", [(65536, 8, 16), (65537, 8, 17), (65536, 8, 32), (65537, 8, 32), (65536, 8, 128), (65537, 8, 128), (131073, 2, 1024), (300001, 8, 4), (300001, 8, 17), (300001, 8, 300)])
 def test_sort_at_tile_sizes(tokens, topk, n):
     """Tiles of each size, with the counts of all tiles added up by every tile or by a launch in between, at both sides of the limit."""
     ids = _ids(np.random.default_rng(tokens + n), tokens, topk, n, "padded")
