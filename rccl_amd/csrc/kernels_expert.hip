@@ -279,73 +279,117 @@ template <typename T> static __device__ __forceinline__ RowCut cutRow(const T* o
 // Which element is a lane's single one, of `singles` in the row.
 static __device__ __forceinline__ uint32_t elementOf(uint32_t head, size_t hidden, uint32_t singles, uint32_t lane) { return lane < head ? lane : (uint32_t)hidden - singles + lane; }
 
-// Dispatch.  A wave takes S slots at a time, V = 8 / S packs in flight for each lane and slot: one slot with rows over 256
-// packs (parts of a row, where there are too few slots to fill the GPU), more with shorter ones.  Long runs of one row are what the
-// time follows: 16384 tokens of 8 slots, 4096 bf16 elements (1.24 GB to move): 8 KiB in one go 0.220 ms, 4 KiB 0.225, 2 KiB
+// Dispatch and the gradient of combine: a workgroup of eight waves takes `each` slots in a row, every lane of a wave loads the
+// position of one, and the waves take the slots that are kept in turn, S rows at a time.
+#define RA_SLOT_WAVES 8
+// What a launch over slots needs before all else, in few 32-bit steps, so that a workgroup without work ends soon.
+struct RaSlots {
+  const int32_t* end;                // how many rows are kept at most (offsets[nExperts]), or null
+  uint32_t slots, rows, groups;      // groups: workgroups of the slots; those behind them clear padding rows
+  uint32_t inverse, shift;           // slot / topk = slot * inverse >> shift, for slots below 2^31
+  uint32_t few[3];                   // `each` doubles where fewer rows than this are kept, and again, and again
+};
+// `each`: 8 S slots where all are kept, so that every wave has a row (S of them), writes it and ends: a wave that goes on to a second row
+// waits for the stores of the first, and with 64 slots in any case 16384 tokens of 8 slots, rows of 8 KiB, take 245 us, with 8 216.
+// More where a rank holds few of the experts and most slots are dropped, so that a wave does not live for one position alone:
+// 65536 tokens of 8 slots, one in eight kept, rows of 8, 4 and 2 KiB 154, 57 and 27 us, a wave for each slot 217, 118
+// and 82 (the gradients 177, 113 and 50 against 312, 291 and 130).  What is kept stands on the device, so the grid fits `rows`
+// and workgroups too many end at once: that is 40 us of the 154.  half: more slots for a workgroup already where half are dropped
+// (dispatch of 16384 tokens of 8 KiB rows 111 us, not so 132; the gradients 184 and 180).
+static RaSlots slotsOf(const RaRowsArgs& a, int S, bool half) {
+  uint32_t l = 0;
+  while ((1 << l) < a.topk) l++;     // 2^(31 + l) / topk, rounded up, is below 2^32; over 2^31 slots its error stays below 1 / topk
+  const uint64_t slots = a.tokens * a.topk;
+  RaSlots n = {a.offsets ? a.offsets + a.nExperts : nullptr, (uint32_t)slots, (uint32_t)a.rows, 0, (uint32_t)(((1ull << (31 + l)) + a.topk - 1) / a.topk), 31 + l, {0, 0, 0}};
+  for (int i = 0; i < 3 && (RA_SLOT_WAVES * S << i) < 64; i++) n.few[i] = (uint32_t)(half && i == 0 ? slots * 3 / 5 : slots / (3 << i)) + 1;
+  return n;
+}
+static __host__ __device__ __forceinline__ uint32_t doublings(const RaSlots& n, uint32_t kept) { return (kept < n.few[0]) + (kept < n.few[1]) + (kept < n.few[2]); }
+template <int S> static __device__ __forceinline__ uint32_t slotsEach(const RaSlots& n) {
+  uint32_t kept = n.rows;
+  if (n.end) { const uint32_t end = (uint32_t)*n.end; kept = end < kept ? end : kept; }
+  return RA_SLOT_WAVES * S << doublings(n, kept);
+}
+// The lanes of the kept slots that are this wave's.
+template <int S> static __device__ __forceinline__ uint64_t sharedOut(bool keep, uint32_t wave) {
+  const uint64_t kept = __ballot(keep);
+  const uint32_t rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(kept >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)kept, 0));
+  return __ballot(keep && rank / S % RA_SLOT_WAVES == wave);
+}
+
+// Dispatch.  V = 8 / S packs in flight for each lane and row: one row with rows over 256 packs (parts of a row, where there are too
+// few slots to fill the GPU), more with shorter ones.  Long runs of one row are what the
+// time follows: 16384 tokens of 8 slots, 4096 bf16 elements (1.24 GB to move): 8 KiB in one go 0.218 ms, 4 KiB 0.225, 2 KiB
 // 0.235; a wave that reads a row once and writes all of the token's rows 0.236, the same through LDS 0.236; streaming accesses
-// 0.225 to 0.250.  The waves of a token's slots are in one workgroup, so that its row comes from HBM once.
-#define RA_SLOT_THREADS 1024         // at most; see slotThreads
+// 0.225 to 0.250.  The waves that write a token's rows are in one workgroup, so that its row comes from HBM once.
 // Sixteen waves of a compute unit at a time: with 20, 24 and 32 the runs of more rows mix, and the time is 0.226, 0.239 and 0.244 ms.
 #define RA_FEW_WAVES(most) __attribute__((amdgpu_waves_per_eu(4, most)))
 template <typename T, int S>
-__global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES(S == 1 ? 4 : 8) void raLocalKernelDispatch(RaRowsArgs a, uint32_t groups, uint32_t parts, uint32_t partElems) {
+__global__ __launch_bounds__(RA_SLOT_WAVES * 64) RA_FEW_WAVES(S == 1 ? 4 : 8) void raLocalKernelDispatch(RaSlots n, RaRowsArgs a, uint32_t parts, uint32_t partElems) {
   constexpr uint32_t N = Pack<T>::N, U = 8, V = S == 1 ? 4 : U / S;      // V: packs of a slot in what is left of its row
-  if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
-  const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63;
-  const size_t slots = a.tokens * a.topk;
-  const uint64_t units = S == 1 ? slots * parts : (slots + S - 1) / S;
-  for (uint64_t unit = (uint64_t)blockIdx.x * waves + uniform(threadIdx.x >> 6); unit < units; unit += (uint64_t)groups * waves) {
-    const size_t slot = S == 1 ? unit / parts : unit * S;
-    const T* x[S];
-    T* out[S];
-    RowCut c[S];
-    bool go[S];
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-      const int32_t pos = slot + s < slots ? a.position[slot + s] : -1;
-      go[s] = pos >= 0 && (size_t)pos < a.rows;
-      x[s] = (const T*)a.in + (size_t)((uint32_t)(slot + s) / (uint32_t)a.topk) * a.inStride;
-      out[s] = (T*)a.out + (size_t)(go[s] ? pos : 0) * a.outStride;
-      c[s] = cutRow(out[s], a.hidden);
-    }
-    uint32_t run = 0;
-    if (S == 1) {
-      if (!go[0]) continue;
-      const uint32_t part = (uint32_t)(unit % parts);
-      run = part * partElems;
-      if (part) c[0].single = 0;                           // (the single elements go with the first part)
-      if (run + partElems < c[0].body) c[0].body = run + partElems;
-    }
-    for (; S == 1 && run + U * 64 * N <= c[0].body; run += U * 64 * N) {
-      u32x4 p[U];
-      const T* from = x[0] + c[0].head + run + lane * N;
-      T* to = out[0] + c[0].head + run + lane * N;
-#pragma unroll
-      for (uint32_t u = 0; u < U; u++) p[u] = wholePack<false>(from + u * 64 * N);
-#pragma unroll
-      for (uint32_t u = 0; u < U; u++) storeWhole<false>(to + u * 64 * N, p[u]);
-    }
-    T single[S];
-    if (S == 1 && lane < c[0].single) single[0] = x[0][elementOf(c[0].head, a.hidden, c[0].single, lane)];
-    do {
-      u32x4 p[S][V];
+  if (blockIdx.x >= n.groups) { padRows<T>(a, blockIdx.x - n.groups); return; }
+  const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const bool split = S == 1 && parts > 1;                              // a wave takes a part of one slot's row
+  const uint32_t each = split ? 1 : slotsEach<S>(n);
+  const uint32_t units = split ? n.slots * parts : (n.slots + each - 1) / each;
+  for (uint32_t unit = split ? blockIdx.x * RA_SLOT_WAVES + wave : blockIdx.x; unit < units; unit += split ? n.groups * RA_SLOT_WAVES : n.groups) {
+    const uint32_t slot = (split ? unit / parts : unit * each) + lane;      // (below 2^31 + 64)
+    int32_t pos = -1;
+    if (lane < each && slot < n.slots) pos = a.position[slot];
+    const uint32_t token = (uint32_t)((uint64_t)slot * n.inverse >> n.shift);
+    const bool keep = pos >= 0 && (uint32_t)pos < n.rows;
+    for (uint64_t kept = split ? __ballot(keep) : sharedOut<S>(keep, wave); kept;) {
+      const T* x[S];
+      T* out[S];
+      RowCut c[S];
+      bool go[S];
 #pragma unroll
       for (int s = 0; s < S; s++) {
-        const T* from = x[s] + c[s].head + run + lane * N;
-#pragma unroll
-        for (uint32_t v = 0; v < V; v++) if (go[s] && run + (v * 64 + lane) * N < c[s].body) p[s][v] = wholePack<false>(from + v * 64 * N);
-        if (S > 1 && go[s] && lane < c[s].single) single[s] = x[s][elementOf(c[s].head, a.hidden, c[s].single, lane)];
+        go[s] = kept != 0;
+        const int k = go[s] ? __builtin_ctzll(kept) : 0;
+        kept &= kept - 1;
+        x[s] = (const T*)a.in + (size_t)(uint32_t)laneInt(token, k) * a.inStride;
+        out[s] = (T*)a.out + (size_t)(go[s] ? laneInt(pos, k) : 0) * a.outStride;
+        c[s] = cutRow(out[s], a.hidden);
       }
-#pragma unroll
-      for (int s = 0; s < S; s++) {
-        T* to = out[s] + c[s].head + run + lane * N;
-#pragma unroll
-        for (uint32_t v = 0; v < V; v++) if (go[s] && run + (v * 64 + lane) * N < c[s].body) storeWhole<false>(to + v * 64 * N, p[s][v]);
-        if (S > 1 && go[s] && lane < c[s].single) out[s][elementOf(c[s].head, a.hidden, c[s].single, lane)] = single[s];
+      uint32_t run = 0;
+      if (split) {
+        const uint32_t part = unit % parts;
+        run = part * partElems;
+        if (part) c[0].single = 0;                           // (the single elements go with the first part)
+        if (run + partElems < c[0].body) c[0].body = run + partElems;
       }
-      run += V * 64 * N;
-    } while (S == 1 && run < c[0].body);
-    if (S == 1 && lane < c[0].single) out[0][elementOf(c[0].head, a.hidden, c[0].single, lane)] = single[0];
+      for (; S == 1 && run + U * 64 * N <= c[0].body; run += U * 64 * N) {
+        u32x4 p[U];
+        const T* from = x[0] + c[0].head + run + lane * N;
+        T* to = out[0] + c[0].head + run + lane * N;
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) p[u] = wholePack<false>(from + u * 64 * N);
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) storeWhole<false>(to + u * 64 * N, p[u]);
+      }
+      T single[S];
+      if (S == 1 && lane < c[0].single) single[0] = x[0][elementOf(c[0].head, a.hidden, c[0].single, lane)];
+      do {
+        u32x4 p[S][V];
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+          const T* from = x[s] + c[s].head + run + lane * N;
+#pragma unroll
+          for (uint32_t v = 0; v < V; v++) if (go[s] && run + (v * 64 + lane) * N < c[s].body) p[s][v] = wholePack<false>(from + v * 64 * N);
+          if (S > 1 && go[s] && lane < c[s].single) single[s] = x[s][elementOf(c[s].head, a.hidden, c[s].single, lane)];
+        }
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+          T* to = out[s] + c[s].head + run + lane * N;
+#pragma unroll
+          for (uint32_t v = 0; v < V; v++) if (go[s] && run + (v * 64 + lane) * N < c[s].body) storeWhole<false>(to + v * 64 * N, p[s][v]);
+          if (S > 1 && go[s] && lane < c[s].single) out[s][elementOf(c[s].head, a.hidden, c[s].single, lane)] = single[s];
+        }
+        run += V * 64 * N;
+      } while (S == 1 && run < c[0].body);
+      if (S == 1 && lane < c[0].single) out[0][elementOf(c[0].head, a.hidden, c[0].single, lane)] = single[0];
+    }
   }
 }
 
@@ -513,77 +557,90 @@ template <typename T> static __device__ __forceinline__ u32x4 gradients(u32x4 z,
 // wave.  Runs of 8 KiB as in dispatch: half of the slots of 16384 tokens (1.17 to 1.38 GB, as routing goes) 6.0 to 6.1 TB/s, a copy
 // has 6.3; runs of 4 KiB 3 % slower, 2 KiB 5 %; a workgroup for each token, its row in registers, no faster.
 template <typename T, int S>
-__global__ __launch_bounds__(RA_SLOT_THREADS) RA_FEW_WAVES(S == 1 ? 4 : 8) void raLocalKernelCombineBackward(RaRowsArgs a, uint32_t groups) {
+__global__ __launch_bounds__(RA_SLOT_WAVES * 64) RA_FEW_WAVES(S == 1 ? 4 : 8) void raLocalKernelCombineBackward(RaSlots n, RaRowsArgs a) {
   constexpr uint32_t N = Pack<T>::N, V = S == 1 ? 4 : 4 / S;      // packs of a slot in what is left of its row
-  if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
-  const uint32_t waves = blockDim.x >> 6, lane = threadIdx.x & 63;
-  const size_t slots = a.tokens * a.topk;
-  for (size_t slot = ((size_t)blockIdx.x * waves + uniform(threadIdx.x >> 6)) * S; slot < slots; slot += (size_t)groups * waves * S) {
-    const T* dy[S];
-    const T* z[S];
-    T* dz[S];
-    RowCut c[S];
-    bool go[S];
-    float w[S], dot[S];
+  if (blockIdx.x >= n.groups) { padRows<T>(a, blockIdx.x - n.groups); return; }
+  const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t each = slotsEach<S>(n);
+  const uint32_t units = (n.slots + each - 1) / each;
+  for (uint32_t unit = blockIdx.x; unit < units; unit += n.groups) {
+    const uint32_t slot = unit * each + lane;
+    const bool exists = lane < each && slot < n.slots;
+    int32_t pos = -1;
+    float weight = 0.f;
+    if (exists) { pos = a.position[slot]; weight = weightOf(a.weights, a.weightType, slot); }
+    const uint32_t token = (uint32_t)((uint64_t)slot * n.inverse >> n.shift);
+    const bool keep = pos >= 0 && (uint32_t)pos < n.rows;
+    if (wave == 0 && exists && !keep) storeWeight(a.dweights, a.weightType, slot, 0.f);
+    for (uint64_t kept = sharedOut<S>(keep, wave); kept;) {
+      const T* dy[S];
+      const T* z[S];
+      T* dz[S];
+      RowCut c[S];
+      bool go[S];
+      uint32_t from[S];
+      float w[S], dot[S];
 #pragma unroll
-    for (int s = 0; s < S; s++) {
-      const bool exists = slot + s < slots;
-      const int32_t pos = exists ? a.position[slot + s] : -1;
-      go[s] = pos >= 0 && (size_t)pos < a.rows;
-      w[s] = go[s] ? weightOf(a.weights, a.weightType, slot + s) : 0.f;
-      dot[s] = 0.f;
-      const size_t row = go[s] ? pos : 0;
-      dy[s] = (const T*)a.in + (size_t)((uint32_t)(slot + s) / (uint32_t)a.topk) * a.inStride;
-      z[s] = (const T*)a.z + row * a.zStride;
-      dz[s] = (T*)a.out + row * a.outStride;
-      c[s] = cutRow(dz[s], a.hidden);
-    }
-    uint32_t run = 0;
-    if (S == 1 && go[0]) {
-      constexpr uint32_t U = 8;
-      for (; run + U * 64 * N <= c[0].body; run += U * 64 * N) {
-        const uint32_t at = c[0].head + run + lane * N;
-        u32x4 p[U], q[U];
+      for (int s = 0; s < S; s++) {
+        go[s] = kept != 0;
+        const int k = go[s] ? __builtin_ctzll(kept) : 0;
+        from[s] = (uint32_t)k;
+        kept &= kept - 1;
+        w[s] = laneFloat(weight, k);
+        dot[s] = 0.f;
+        const size_t row = go[s] ? laneInt(pos, k) : 0;
+        dy[s] = (const T*)a.in + (size_t)(uint32_t)laneInt(token, k) * a.inStride;
+        z[s] = (const T*)a.z + row * a.zStride;
+        dz[s] = (T*)a.out + row * a.outStride;
+        c[s] = cutRow(dz[s], a.hidden);
+      }
+      uint32_t run = 0;
+      if (S == 1) {
+        constexpr uint32_t U = 8;
+        for (; run + U * 64 * N <= c[0].body; run += U * 64 * N) {
+          const uint32_t at = c[0].head + run + lane * N;
+          u32x4 p[U], q[U];
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) { p[u] = wholePack<true>(z[0] + at + u * 64 * N); q[u] = wholePack<false>(dy[0] + at + u * 64 * N); }
+          for (uint32_t u = 0; u < U; u++) { p[u] = wholePack<true>(z[0] + at + u * 64 * N); q[u] = wholePack<false>(dy[0] + at + u * 64 * N); }
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) {
-          storeWhole<true>(dz[0] + at + u * 64 * N, gradients<T>(p[u], q[u], w[0], dot[0]));
-          __builtin_amdgcn_sched_barrier(0);               // one pack as floats at a time: the packs take half of the registers
+          for (uint32_t u = 0; u < U; u++) {
+            storeWhole<true>(dz[0] + at + u * 64 * N, gradients<T>(p[u], q[u], w[0], dot[0]));
+            __builtin_amdgcn_sched_barrier(0);               // one pack as floats at a time: the packs take half of the registers
+          }
         }
       }
-    }
-    do {
-      u32x4 p[S][V], q[S][V];
+      do {
+        u32x4 p[S][V], q[S][V];
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+          const uint32_t at = c[s].head + run + lane * N;
+#pragma unroll
+          for (uint32_t v = 0; v < V; v++)
+            if (go[s] && run + (v * 64 + lane) * N < c[s].body) { p[s][v] = wholePack<true>(z[s] + at + v * 64 * N); q[s][v] = wholePack<false>(dy[s] + at + v * 64 * N); }
+        }
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+          const uint32_t at = c[s].head + run + lane * N;
+#pragma unroll
+          for (uint32_t v = 0; v < V; v++)
+            if (go[s] && run + (v * 64 + lane) * N < c[s].body) storeWhole<true>(dz[s] + at + v * 64 * N, gradients<T>(p[s][v], q[s][v], w[s], dot[s]));
+        }
+        run += V * 64 * N;
+      } while (S == 1 && run < c[0].body);
 #pragma unroll
       for (int s = 0; s < S; s++) {
-        const uint32_t at = c[s].head + run + lane * N;
-#pragma unroll
-        for (uint32_t v = 0; v < V; v++)
-          if (go[s] && run + (v * 64 + lane) * N < c[s].body) { p[s][v] = wholePack<true>(z[s] + at + v * 64 * N); q[s][v] = wholePack<false>(dy[s] + at + v * 64 * N); }
+        if (go[s] && lane < c[s].single) {
+          const uint32_t i = elementOf(c[s].head, a.hidden, c[s].single, lane);
+          const float d = (float)dy[s][i];
+          dot[s] = __builtin_fmaf(d, (float)z[s][i], dot[s]);
+          dz[s][i] = (T)(w[s] * d);
+        }
       }
 #pragma unroll
       for (int s = 0; s < S; s++) {
-        const uint32_t at = c[s].head + run + lane * N;
-#pragma unroll
-        for (uint32_t v = 0; v < V; v++)
-          if (go[s] && run + (v * 64 + lane) * N < c[s].body) storeWhole<true>(dz[s] + at + v * 64 * N, gradients<T>(p[s][v], q[s][v], w[s], dot[s]));
+        const float sum = laneFloat(waveSum63(dot[s]), 63);
+        if (go[s] && lane == from[s]) storeWeight(a.dweights, a.weightType, slot, sum);
       }
-      run += V * 64 * N;
-    } while (S == 1 && go[0] && run < c[0].body);
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-      if (go[s] && lane < c[s].single) {
-        const uint32_t i = elementOf(c[s].head, a.hidden, c[s].single, lane);
-        const float d = (float)dy[s][i];
-        dot[s] = __builtin_fmaf(d, (float)z[s][i], dot[s]);
-        dz[s][i] = (T)(w[s] * d);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-      const float sum = waveSum63(dot[s]);
-      if (lane == 63 && slot + s < slots) storeWeight(a.dweights, a.weightType, slot + s, sum);
     }
   }
 }
@@ -611,14 +668,15 @@ __global__ __launch_bounds__(RA_NARROW_THREADS) void raLocalKernelCombineBackwar
 
 static uint32_t padGroups(const RaRowsArgs& a) { return a.offsets ? (uint32_t)a.nExperts * RA_PAD_GROUPS : 0; }
 
-// Threads of a workgroup of slots: whole tokens, eight waves or nearly so.
-static int slotThreads(int topk) { return 64 * (topk <= 8 ? 8 / topk * topk : topk <= 16 ? topk : 8); }
 // Workgroups for so many waves: one each, up to 2^20 workgroups, beyond which a wave takes several in turn (a launch has fewer
 // than 2^32 threads).
 static uint32_t groupsOf(uint64_t units, int threads) {
   const uint64_t g = (units + threads / 64 - 1) / (threads / 64);
   return (uint32_t)(g < 1u << 20 ? g : 1u << 20);
 }
+
+// Workgroups for slots of which as many may be kept as there are rows.
+static uint32_t slotGroups(const RaSlots& n, int S) { return groupsOf((((uint64_t)n.slots - 1) >> doublings(n, n.rows)) / (RA_SLOT_WAVES * S) + 1, 64); }
 
 // Lanes for a row of few packs, as a power of two; 6 (a whole wave): the row is not narrow.
 template <typename T> static uint32_t narrowShift(const RaRowsArgs& a) {
@@ -627,28 +685,29 @@ template <typename T> static uint32_t narrowShift(const RaRowsArgs& a) {
   return shift;
 }
 template <typename T, int S>
-static hipError_t launchDispatch(const RaRowsArgs& a, uint32_t groups, int threads, uint32_t parts, uint32_t partElems, hipStream_t s) {
-  return raLaunch(raLocalKernelDispatch<T, S>, groups + padGroups(a), threads, 0, s, a, groups, parts, partElems);
+static hipError_t launchDispatch(const RaRowsArgs& a, uint32_t parts, uint32_t partElems, hipStream_t s) {
+  RaSlots n = slotsOf(a, S, true);
+  n.groups = n.slots == 0 ? 0 : parts > 1 ? groupsOf((uint64_t)n.slots * parts, RA_SLOT_WAVES * 64) : slotGroups(n, S);
+  return raLaunch(raLocalKernelDispatch<T, S>, n.groups + padGroups(a), RA_SLOT_WAVES * 64, 0, s, n, a, parts, partElems);
 }
 template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_t s) {
   const uint32_t shift = narrowShift<T>(a);
+  const uint64_t slots = (uint64_t)a.tokens * a.topk, step = 64 * Pack<T>::N;
   if (shift < 6) {
-    const uint32_t groups = groupsOf(((uint64_t)a.tokens * a.topk + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS);
+    const uint32_t groups = groupsOf((slots + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS);
     return raLaunch(raLocalKernelDispatchNarrow<T>, groups + padGroups(a), RA_NARROW_THREADS, 0, s, a, groups, shift);
   }
-  const uint64_t slots = (uint64_t)a.tokens * a.topk, step = 64 * Pack<T>::N;
-  const int threads = slotThreads(a.topk);
   // Short rows: several slots for a wave, where that leaves 4096 waves
   const uint64_t runs = (a.hidden + step - 1) / step;
-  if (runs <= 1 && slots >= 8 * 4096) return launchDispatch<T, 8>(a, groupsOf((slots + 7) / 8, threads), threads, 1, 0, s);
-  if (runs <= 2 && slots >= 4 * 4096) return launchDispatch<T, 4>(a, groupsOf((slots + 3) / 4, threads), threads, 1, 0, s);
-  if (runs <= 4 && slots >= 2 * 4096) return launchDispatch<T, 2>(a, groupsOf((slots + 1) / 2, threads), threads, 1, 0, s);
+  if (runs <= 1 && slots >= 8 * 4096) return launchDispatch<T, 8>(a, 1, 0, s);
+  if (runs <= 2 && slots >= 4 * 4096) return launchDispatch<T, 4>(a, 1, 0, s);
+  if (runs <= 4 && slots >= 2 * 4096) return launchDispatch<T, 2>(a, 1, 0, s);
   // parts of a row, down to 64 packs, where there are fewer than 4096 waves otherwise
   uint64_t parts = 1;
   while (parts < runs && slots * parts < 4096) parts *= 2;
   const uint64_t partElems = ((a.hidden + parts - 1) / parts + step - 1) / step * step;
   parts = (a.hidden + partElems - 1) / partElems;
-  return launchDispatch<T, 1>(a, groupsOf(slots * parts, threads), threads, (uint32_t)parts, (uint32_t)partElems, s);
+  return launchDispatch<T, 1>(a, (uint32_t)parts, (uint32_t)partElems, s);
 }
 template <typename T> static hipError_t combine(const RaRowsArgs& a, hipStream_t s) {
   const uint32_t shift = narrowShift<T>(a);
@@ -667,13 +726,14 @@ template <typename T> static hipError_t combineBackward(const RaRowsArgs& a, hip
     const uint32_t groups = groupsOf(((uint64_t)a.tokens * a.topk + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS);
     return raLaunch(raLocalKernelCombineBackwardNarrow<T>, groups + padGroups(a), RA_NARROW_THREADS, 0, s, a, groups, shift);
   }
-  const int threads = slotThreads(a.topk);
   const uint64_t slots = (uint64_t)a.tokens * a.topk, runs = (a.hidden + 64 * Pack<T>::N - 1) / (64 * Pack<T>::N);
-  const int each = runs <= 1 && slots >= 4096 * 4 ? 4 : runs <= 2 && slots >= 4096 * 2 ? 2 : 1;
-  const uint32_t groups = groupsOf((slots + each - 1) / each, threads);
-  return each == 4 ? raLaunch(raLocalKernelCombineBackward<T, 4>, groups + padGroups(a), threads, 0, s, a, groups)
-       : each == 2 ? raLaunch(raLocalKernelCombineBackward<T, 2>, groups + padGroups(a), threads, 0, s, a, groups)
-                   : raLaunch(raLocalKernelCombineBackward<T, 1>, groups + padGroups(a), threads, 0, s, a, groups);
+  const int at = runs <= 1 && slots >= 4096 * 4 ? 4 : runs <= 2 && slots >= 4096 * 2 ? 2 : 1;
+  RaSlots n = slotsOf(a, at, false);
+  n.groups = n.slots ? slotGroups(n, at) : 0;
+  const uint32_t groups = n.groups + padGroups(a);
+  return at == 4 ? raLaunch(raLocalKernelCombineBackward<T, 4>, groups, RA_SLOT_WAVES * 64, 0, s, n, a)
+       : at == 2 ? raLaunch(raLocalKernelCombineBackward<T, 2>, groups, RA_SLOT_WAVES * 64, 0, s, n, a)
+                 : raLaunch(raLocalKernelCombineBackward<T, 1>, groups, RA_SLOT_WAVES * 64, 0, s, n, a);
 }
 #define RA_BY_TYPE(fn)                                    \
   switch (type) {                                         \

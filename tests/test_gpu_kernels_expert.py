@@ -321,6 +321,49 @@ def test_short_rows_of_many_slots(topk, tokens, hidden, dtype, gap, shift):
     assert torch.all((dw.double() - prod.sum(2)).abs() <= 1.01 * (hidden // 64 + 14) * ref.U * prod.abs().sum(2) + ref.TINY["f32"])
 
 
+@pytest.mark.parametrize("hidden,dtype", [(512, "bf16"), (1000, "f16"), (1024, "f32"), (4104, "bf16")])
+@pytest.mark.parametrize("n", [0, 1, 3, 6, 12, 24, 36, 64])
+@pytest.mark.parametrize("how", ["offsets", "rows", "neither"])
+def test_dropped_slots(hidden, dtype, n, how):
+    """A rank that holds n of 64 experts (0: one that nobody chose): all, some or almost none of the slots are kept, which the
+    offsets, the number of rows or only the positions say."""
+    import torch
+    import rccl_amd as ra
+    gen = torch.Generator("cuda").manual_seed(hidden + n)
+    code, tt = _types()[dtype]
+    tokens, topk = 4500 if hidden < 2000 else 1100, 8
+    ids = torch.randint(0, 64, (tokens, topk), device="cuda", generator=gen)
+    n, first = (n, 0) if n else (1, 64)
+    pos, off, cnt = (torch.empty(k, dtype=torch.int32, device="cuda") for k in (tokens * topk, n + 1, n))
+    work = torch.empty(ra.expert_sort_bytes(tokens, topk, n), dtype=torch.uint8, device="cuda")
+    ra.expert_sort(ids, ra.ncclInt64, tokens, topk, first, n, 4, pos, None, off, cnt, work)
+    keep = pos >= 0
+    assert torch.equal(keep, ((ids >= first) & (ids < first + n)).view(-1))
+    held = int(off[-1])
+    rows = held + 3 if how == "rows" else ra.expert_rows(tokens, topk, n, 4)
+    segments = dict(offsets=off, counts=cnt, n_experts=n) if how == "offsets" else {}
+    token = torch.arange(tokens * topk, device="cuda") // topk
+    x, dy = (torch.randn(tokens, hidden, device="cuda", generator=gen).to(tt) for _ in range(2))
+    z = torch.randn(rows, hidden, device="cuda", generator=gen).to(tt)
+    w = torch.randn(tokens, topk, device="cuda", generator=gen)
+    out, dz, dw = torch.full((rows, hidden), 5.0, dtype=tt, device="cuda"), torch.full((rows, hidden), 5.0, dtype=tt, device="cuda"), torch.full((tokens, topk), 9.0, device="cuda")
+    ra.expert_dispatch(x, out, rows, code, tokens, topk, hidden, pos, **segments)
+    ra.expert_combine_backward(dy, z, rows, w, ra.ncclFloat32, dz, dw, code, tokens, topk, hidden, pos, **segments)
+    at = pos[keep].long()
+    want, wantz = torch.full((rows, hidden), 5.0, dtype=tt, device="cuda"), torch.full((rows, hidden), 5.0, dtype=torch.float64, device="cuda")
+    if how == "offsets":
+        want[:held], wantz[:held] = 0.0, 0.0
+    want[at] = x[token[keep]]
+    assert torch.equal(out, want)
+    half = ref.HALF_STEP[dtype] if dtype != "f32" else 0.0
+    wantz[at] = dy[token[keep]].double() * w.view(-1)[keep, None].double()
+    assert torch.all((dz.double() - wantz).abs() <= (1.01 * ref.U + 1.01 * half) * wantz.abs() + ref.TINY[dtype])
+    prod = dy[token[keep]].double() * z[at].double()
+    # a lane adds the products of its part of the row (a 64th of it, in packs of at most 8 elements), then 6 sums join them
+    assert torch.all((dw.view(-1)[keep].double() - prod.sum(1)).abs() <= 1.01 * (hidden // 64 + 14) * ref.U * prod.abs().sum(1) + ref.TINY["f32"])
+    assert torch.all(dw.view(-1)[~keep] == 0.0)
+
+
 def test_gradients_against_differences():
     """<dy, combine(z, w)> is linear in z and in w: its differences are exact up to rounding, in fp32 with small whole numbers
     exactly.  The gradient of a dispatch is a combine without weights: <dout, dispatch(x)> = <combine(dout), x>."""
