@@ -393,18 +393,47 @@ __global__ __launch_bounds__(RA_SLOT_WAVES * 64) RA_FEW_WAVES(S == 1 ? 4 : 8) vo
   }
 }
 
-// Rows of at most 32 packs: a group of `1 << shift` lanes takes one, so that a wave moves several at a time.
+// Rows of at most 32 packs: a group of `1 << shift` lanes takes one, so that a wave moves several at a time, and each lane one
+// of two rows at a time where there are many (524288 slots of 128 bf16, gradients: 53 us, one 58, four 64).
 #define RA_NARROW_THREADS 256
-template <typename T>
+#define RA_NARROW_ROWS 2
+// A lane's pack of a narrow row.  The last one ends where the row ends and so repeats elements of the one before it (`twice`), which
+// both lanes read and write alike (the lanes of a row are one wave's: all have read before one writes).  Rows of 100 elements take 25, 28 and 83 us
+// for dispatch, combine and its gradients this way, 39, 47 and 108 with single elements at the end.  !WHOLE: a row shorter than a
+// pack, moved element by element.
+template <typename T, bool WHOLE> struct Narrow {
+  size_t at; int twice; bool any;
+  __device__ __forceinline__ Narrow(size_t hidden, uint32_t shift) {
+    constexpr int N = Pack<T>::N;
+    at = (threadIdx.x & ((1u << shift) - 1)) * N;
+    any = at < hidden;
+    twice = WHOLE && any && at + N > hidden ? (int)(at + N - hidden) : 0;
+    at -= twice;
+  }
+  template <bool STREAM> __device__ __forceinline__ u32x4 load(const T* row, size_t hidden) const { return WHOLE ? wholePack<STREAM>(row + at) : loadPack<STREAM>(row, at, hidden); }
+  template <bool STREAM> __device__ __forceinline__ void store(T* row, size_t hidden, u32x4 p) const {
+    if (WHOLE) storeWhole<STREAM>(row + at, p);
+    else storePack<STREAM>(row, at, hidden, p);
+  }
+};
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(RA_NARROW_THREADS) void raLocalKernelDispatchNarrow(RaRowsArgs a, uint32_t groups, uint32_t shift) {
-  constexpr int N = Pack<T>::N;
+  constexpr int F = RA_NARROW_ROWS;
   if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
   const size_t slots = a.tokens * a.topk, step = (size_t)groups * RA_NARROW_THREADS >> shift;
-  const size_t at = (threadIdx.x & ((1u << shift) - 1)) * N;
-  for (size_t slot = ((size_t)blockIdx.x * RA_NARROW_THREADS + threadIdx.x) >> shift; slot < slots; slot += step) {
-    const int32_t pos = a.position[slot];
-    if (pos < 0 || (size_t)pos >= a.rows || at >= a.hidden) continue;
-    storePack<false>((T*)a.out + (size_t)pos * a.outStride, at, a.hidden, loadPack<false>((const T*)a.in + (size_t)((uint32_t)slot / (uint32_t)a.topk) * a.inStride, at, a.hidden));
+  const Narrow<T, WHOLE> mine(a.hidden, shift);
+  if (!mine.any) return;
+  for (size_t slot = ((size_t)blockIdx.x * RA_NARROW_THREADS + threadIdx.x) >> shift; slot < slots; slot += F * step) {
+    int32_t pos[F];
+    u32x4 p[F];
+#pragma unroll
+    for (int f = 0; f < F; f++) pos[f] = slot + f * step < slots ? a.position[slot + f * step] : -1;
+#pragma unroll
+    for (int f = 0; f < F; f++)
+      if (pos[f] >= 0 && (size_t)pos[f] < a.rows) p[f] = mine.template load<false>((const T*)a.in + (size_t)((uint32_t)(slot + f * step) / (uint32_t)a.topk) * a.inStride, a.hidden);
+#pragma unroll
+    for (int f = 0; f < F; f++)
+      if (pos[f] >= 0 && (size_t)pos[f] < a.rows) mine.template store<false>((T*)a.out + (size_t)pos[f] * a.outStride, a.hidden, p[f]);
   }
 }
 
@@ -498,12 +527,13 @@ __global__ __launch_bounds__(RA_COMBINE_THREADS) void raLocalKernelCombine(RaRow
 }
 
 // Rows of at most 32 packs: `1 << shift` lanes for each token.
-template <typename T>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(RA_NARROW_THREADS) void raLocalKernelCombineNarrow(RaRowsArgs a, uint32_t shift) {
   constexpr int N = Pack<T>::N, F = 4;
   typedef typename Pack<T>::floats floats;
-  const size_t step = (size_t)gridDim.x * RA_NARROW_THREADS >> shift, at = (threadIdx.x & ((1u << shift) - 1)) * N;
-  if (at >= a.hidden) return;
+  const size_t step = (size_t)gridDim.x * RA_NARROW_THREADS >> shift;
+  const Narrow<T, WHOLE> mine(a.hidden, shift);
+  if (!mine.any) return;
   for (size_t token = ((size_t)blockIdx.x * RA_NARROW_THREADS + threadIdx.x) >> shift; token < a.tokens; token += step) {
     floats sum = {};
     for (int k = 0; k < a.topk; k += F) {
@@ -518,7 +548,7 @@ __global__ __launch_bounds__(RA_NARROW_THREADS) void raLocalKernelCombineNarrow(
         const int32_t pos = a.position[slot];
         if (pos < 0 || (size_t)pos >= a.rows) continue;
         w[f] = a.weightType >= 0 ? weightOf(a.weights, a.weightType, slot) : 1.f;
-        p[f] = loadPack<true>((const T*)a.in + (size_t)pos * a.inStride, at, a.hidden);
+        p[f] = mine.template load<true>((const T*)a.in + (size_t)pos * a.inStride, a.hidden);
       }
 #pragma unroll
       for (int f = 0; f < F; f++) {                        // (a slot that is not there adds 0 * 0)
@@ -527,7 +557,7 @@ __global__ __launch_bounds__(RA_NARROW_THREADS) void raLocalKernelCombineNarrow(
         for (int i = 0; i < N; i++) sum[i] = __builtin_fmaf(w[f], z[i], sum[i]);
       }
     }
-    storePack<true>((T*)a.out + token * a.outStride, at, a.hidden, fromFloats<T>(sum));
+    mine.template store<true>((T*)a.out + token * a.outStride, a.hidden, fromFloats<T>(sum));
   }
 }
 
@@ -646,23 +676,43 @@ __global__ __launch_bounds__(RA_SLOT_WAVES * 64) RA_FEW_WAVES(S == 1 ? 4 : 8) vo
 }
 
 // Rows of at most 32 packs: `1 << shift` lanes for each slot.
-template <typename T>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(RA_NARROW_THREADS) void raLocalKernelCombineBackwardNarrow(RaRowsArgs a, uint32_t groups, uint32_t shift) {
-  constexpr int N = Pack<T>::N;
+  constexpr int N = Pack<T>::N, F = RA_NARROW_ROWS;
   if (blockIdx.x >= groups) { padRows<T>(a, blockIdx.x - groups); return; }
   const size_t slots = a.tokens * a.topk, step = (size_t)groups * RA_NARROW_THREADS >> shift;
-  const size_t at = (threadIdx.x & ((1u << shift) - 1)) * N;
-  for (size_t slot = ((size_t)blockIdx.x * RA_NARROW_THREADS + threadIdx.x) >> shift; slot < slots; slot += step) {
-    const int32_t pos = a.position[slot];
-    float dot = 0.f;
-    if (pos >= 0 && (size_t)pos < a.rows && at < a.hidden) {
-      const float w = weightOf(a.weights, a.weightType, slot);
-      const u32x4 d = loadPack<false>((const T*)a.in + (size_t)((uint32_t)slot / (uint32_t)a.topk) * a.inStride, at, a.hidden);
-      const u32x4 z = loadPack<true>((const T*)a.z + (size_t)pos * a.zStride, at, a.hidden);
-      storePack<true>((T*)a.out + (size_t)pos * a.outStride, at, a.hidden, gradients<T>(z, d, w, dot));
+  const Narrow<T, WHOLE> mine(a.hidden, shift);
+  for (size_t slot = ((size_t)blockIdx.x * RA_NARROW_THREADS + threadIdx.x) >> shift; slot < slots; slot += F * step) {
+    int32_t pos[F];
+    float w[F], dot[F];
+    u32x4 p[F], q[F];
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      pos[f] = slot + f * step < slots ? a.position[slot + f * step] : -1;
+      if ((size_t)(uint32_t)pos[f] >= a.rows) pos[f] = -1;
+      dot[f] = 0.f;
     }
-    for (int s = 1; s < 1 << shift; s <<= 1) dot += __shfl_xor(dot, s);      // (the lanes of a slot run together)
-    if (at == 0) storeWeight(a.dweights, a.weightType, slot, dot);
+#pragma unroll
+    for (int f = 0; f < F; f++)
+      if (pos[f] >= 0 && mine.any) {
+        w[f] = weightOf(a.weights, a.weightType, slot + f * step);
+        q[f] = mine.template load<false>((const T*)a.in + (size_t)((uint32_t)(slot + f * step) / (uint32_t)a.topk) * a.inStride, a.hidden);
+        p[f] = mine.template load<true>((const T*)a.z + (size_t)pos[f] * a.zStride, a.hidden);
+      }
+#pragma unroll
+    for (int f = 0; f < F; f++)
+      if (pos[f] >= 0 && mine.any) {
+        const typename Pack<T>::floats z = toFloats<T>(p[f]), d = toFloats<T>(q[f]);
+        typename Pack<T>::floats g;
+#pragma unroll
+        for (int i = 0; i < N; i++) { dot[f] = i >= mine.twice ? __builtin_fmaf(d[i], z[i], dot[f]) : dot[f]; g[i] = w[f] * d[i]; }
+        mine.template store<true>((T*)a.out + (size_t)pos[f] * a.outStride, a.hidden, fromFloats<T>(g));
+      }
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      for (int s = 1; s < 1 << shift; s <<= 1) dot[f] += __shfl_xor(dot[f], s);      // (the lanes of a slot run together)
+      if ((threadIdx.x & ((1u << shift) - 1)) == 0 && slot + f * step < slots) storeWeight(a.dweights, a.weightType, slot + f * step, dot[f]);
+    }
   }
 }
 
@@ -677,6 +727,12 @@ static uint32_t groupsOf(uint64_t units, int threads) {
 
 // Workgroups for slots of which as many may be kept as there are rows.
 static uint32_t slotGroups(const RaSlots& n, int S) { return groupsOf((((uint64_t)n.slots - 1) >> doublings(n, n.rows)) / (RA_SLOT_WAVES * S) + 1, 64); }
+
+// Workgroups for narrow rows: two rows for each lane where that leaves 8192 waves.
+static uint32_t narrowGroups(uint64_t rows, uint32_t shift) {
+  const uint64_t waves = (rows + (63 >> shift)) >> (6 - shift);
+  return groupsOf(waves >= 8192 * RA_NARROW_ROWS ? (waves + RA_NARROW_ROWS - 1) / RA_NARROW_ROWS : waves, RA_NARROW_THREADS);
+}
 
 // Lanes for a row of few packs, as a power of two; 6 (a whole wave): the row is not narrow.
 template <typename T> static uint32_t narrowShift(const RaRowsArgs& a) {
@@ -694,8 +750,8 @@ template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_
   const uint32_t shift = narrowShift<T>(a);
   const uint64_t slots = (uint64_t)a.tokens * a.topk, step = 64 * Pack<T>::N;
   if (shift < 6) {
-    const uint32_t groups = groupsOf((slots + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS);
-    return raLaunch(raLocalKernelDispatchNarrow<T>, groups + padGroups(a), RA_NARROW_THREADS, 0, s, a, groups, shift);
+    const uint32_t groups = narrowGroups(slots, shift);
+    return raLaunch(a.hidden >= Pack<T>::N ? raLocalKernelDispatchNarrow<T, true> : raLocalKernelDispatchNarrow<T, false>, groups + padGroups(a), RA_NARROW_THREADS, 0, s, a, groups, shift);
   }
   // Short rows: several slots for a wave, where that leaves 4096 waves
   const uint64_t runs = (a.hidden + step - 1) / step;
@@ -712,7 +768,7 @@ template <typename T> static hipError_t dispatch(const RaRowsArgs& a, hipStream_
 template <typename T> static hipError_t combine(const RaRowsArgs& a, hipStream_t s) {
   const uint32_t shift = narrowShift<T>(a);
   if (shift < 6) {
-    return raLaunch(raLocalKernelCombineNarrow<T>, groupsOf((a.tokens + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS), RA_NARROW_THREADS, 0, s, a, shift);
+    return raLaunch(a.hidden >= Pack<T>::N ? raLocalKernelCombineNarrow<T, true> : raLocalKernelCombineNarrow<T, false>, groupsOf((a.tokens + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS), RA_NARROW_THREADS, 0, s, a, shift);
   }
   const uint64_t step = 64 * Pack<T>::N;
   // four runs of 64 packs for each wave, or one where that leaves fewer than 4096 waves
@@ -723,8 +779,8 @@ template <typename T> static hipError_t combine(const RaRowsArgs& a, hipStream_t
 template <typename T> static hipError_t combineBackward(const RaRowsArgs& a, hipStream_t s) {
   const uint32_t shift = narrowShift<T>(a);
   if (shift < 6) {
-    const uint32_t groups = groupsOf(((uint64_t)a.tokens * a.topk + (63 >> shift)) >> (6 - shift), RA_NARROW_THREADS);
-    return raLaunch(raLocalKernelCombineBackwardNarrow<T>, groups + padGroups(a), RA_NARROW_THREADS, 0, s, a, groups, shift);
+    const uint32_t groups = narrowGroups((uint64_t)a.tokens * a.topk, shift);
+    return raLaunch(a.hidden >= Pack<T>::N ? raLocalKernelCombineBackwardNarrow<T, true> : raLocalKernelCombineBackwardNarrow<T, false>, groups + padGroups(a), RA_NARROW_THREADS, 0, s, a, groups, shift);
   }
   const uint64_t slots = (uint64_t)a.tokens * a.topk, runs = (a.hidden + 64 * Pack<T>::N - 1) / (64 * Pack<T>::N);
   const int at = runs <= 1 && slots >= 4096 * 4 ? 4 : runs <= 2 && slots >= 4096 * 2 ? 2 : 1;

@@ -172,7 +172,7 @@ def _np64(t):
 
 ROWS = [(1, 1, 1, "bf16", 0, 0), (1, 8, 4096, "bf16", 0, 0), (3, 2, 7, "bf16", 1, 1), (65, 2, 8, "f16", 0, 0), (64, 3, 9, "f32", 3, 1), (130, 8, 63, "f16", 5, 3),
         (77, 6, 512, "bf16", 8, 0), (50, 64, 130, "bf16", 0, 2), (33, 4, 1000, "f32", 24, 0), (40, 5, 1001, "f32", 0, 0), (300, 2, 2048, "f16", 0, 0),
-        (19, 8, 4097, "bf16", 7, 1), (9, 8, 8200, "f32", 0, 0), (5, 3, 33000, "bf16", 0, 0), (2000, 4, 16, "bf16", 0, 0)]
+        (19, 8, 4097, "bf16", 7, 1), (9000, 4, 100, "bf16", 0, 1), (9000, 4, 70, "f32", 1, 0), (20001, 3, 129, "f16", 0, 0), (30000, 2, 5, "bf16", 0, 0), (9, 8, 8200, "f32", 0, 0), (5, 3, 33000, "bf16", 0, 0), (2000, 4, 16, "bf16", 0, 0)]
 
 
 @pytest.mark.parametrize("tokens,topk,hidden,dtype,gap,shift", ROWS)
