@@ -356,7 +356,8 @@ ncclResult_t rcclAmdExpertSortBytes(size_t tokens, int topk, int nExperts, size_
  * elements apart; `out` has `rows` rows, and positions outside 0 .. rows - 1 are passed over.  Two slots may not name the
  * same row.  With offsets and counts
  * (both or neither, as rcclAmdExpertSort gives them) the padding rows offsets[e] + counts[e] .. offsets[e + 1] - 1 are set to
- * zero; all other rows without a slot are left as they were.  Its gradient with respect to x is rcclAmdExpertCombine of
+ * zero; all other rows without a slot are left as they were.  (offsets, or else `rows`, also say how the work is best shared out
+ * where most slots are dropped; results do not depend on it.)  Its gradient with respect to x is rcclAmdExpertCombine of
  * the gradient of out, without weights. */
 ncclResult_t rcclAmdExpertDispatch(const void* x, size_t xStride, void* out, size_t outStride, size_t rows,
                                    ncclDataType_t datatype, size_t tokens, int topk, size_t hidden, const int32_t* position,
