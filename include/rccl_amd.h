@@ -298,7 +298,7 @@ typedef struct {
   const void* grad;          /* gradType */
   void* expAvg;              /* float, or e4m3 bytes */
   void* expAvgSq;
-  uint8_t* expAvgScale;      /* rcclAmdStateMx8 only: ceil(count / 32) bytes each */
+  uint8_t* expAvgScale;      /* rcclAmdStateMx8: ceil(count / 32) bytes each; rcclAmdStateF32: NULL */
   uint8_t* expAvgSqScale;
   void* copy;                /* NULL, or where the updated parameter is written once more, rounded to copyType */
   size_t count;              /* elements; 0 is allowed and does nothing */

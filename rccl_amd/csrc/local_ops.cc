@@ -94,6 +94,8 @@ RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntenso
     if (t.count == 0) continue;
     if (t.count > kMaxElements || (all += t.count) > kMaxElements) RA_REFUSE("%s: tensor %d: %zu elements, or too many in all", fn, i, t.count);
     if (!t.param || !t.grad || !t.expAvg || !t.expAvgSq || (mx && (!t.expAvgScale || !t.expAvgSqScale))) RA_REFUSE("%s: tensor %d has a null buffer", fn, i);
+    // (what has scales has moments of one byte: taken for floats they would be read and written far past their end)
+    if (!mx && (t.expAvgScale || t.expAvgSqScale)) RA_REFUSE("%s: tensor %d has scales, which 32-bit states have not", fn, i);
     if (!aligned(t.param, ps) || !aligned(t.grad, gs) || (!mx && (!aligned(t.expAvg, 4) || !aligned(t.expAvgSq, 4))) || !aligned(t.copy, cs))
       RA_REFUSE("%s: tensor %d has a buffer that is not aligned to its element type", fn, i);
     copies = copies || t.copy;

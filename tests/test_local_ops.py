@@ -44,6 +44,14 @@ def test_adamw_refuses_an_eps_that_fp32_does_not_hold_as_a_normal_number(eps):
     _refused(lambda: _adamw(eps=eps), "normal fp32")
 
 
+@pytest.mark.parametrize("scales", [(P, P), (P, 0), (0, P)])
+@pytest.mark.parametrize("ntensors", [1, 200])
+def test_adamw_refuses_8_bit_moments_as_floats(scales, ntensors):
+    """A row with scales names moments of one byte each; with 32-bit states they would be read and written past their end."""
+    rows = [[P, P, P, P, *(scales if i == ntensors - 1 else (0, 0)), 0, 100] for i in range(ntensors)]
+    _refused(lambda: _adamw(rows=rows), "has scales")
+
+
 def test_adamw_without_work():
     _adamw(rows=np.zeros((0, 8)))
     _adamw(rows=[[0] * 8] * 200)                               # empty tensors need no buffers
