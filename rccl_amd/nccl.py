@@ -563,11 +563,13 @@ def sum_squares(tensors, counts, datatype, out, workspace, accumulate=False, str
         rc = (_mirror or _bind()).sum_squares(tensors, counts, datatype, out, workspace, accumulate, stream)
         if rc >= 0:
             return _check(rc, where)
-    if isinstance(tensors, (list, tuple)) and tensors and hasattr(tensors[0], "data_ptr"):
-        counts = [t.numel() for t in tensors] if counts is None else counts
-        tensors = [_whole(t, n, datatype, where, "a tensor") for t, n in zip(tensors, counts)]
+    own = isinstance(tensors, (list, tuple)) and tensors and hasattr(tensors[0], "data_ptr")
+    if own and counts is None:
+        counts = [t.numel() for t in tensors]
     if counts is None or len(counts) != len(tensors):
         _refuse(where, f"{len(tensors)} tensors with other counts")
+    if own:
+        tensors = [_whole(t, n, datatype, where, "a tensor") for t, n in zip(tensors, counts)]
     ptrs, n, keep = _host_table(tensors, None, where) if len(tensors) else (None, 0, None)
     sizes, _, keep2 = _host_table(counts, None, where) if len(tensors) else (None, 0, None)
     w, nbytes = _work(workspace, sum_squares_bytes(n) if isinstance(workspace, int) else 0, where)

@@ -83,6 +83,39 @@ def test_sum_squares_refusals():
     assert L.rcclAmdSumSquaresBytes(1, None) == ra.ncclInvalidArgument
 
 
+class _Tensor:
+    """What the checks of a tensor ask, of one that lies on the current device."""
+    def __init__(self, n, dtype):
+        self.n, self.dtype = n, dtype
+
+    def data_ptr(self):
+        return P
+
+    def numel(self):
+        return self.n
+
+    def get_device(self):
+        return 0
+
+    def is_contiguous(self):
+        return True
+
+
+@pytest.mark.parametrize("counts", [[5], [], [5, 5, 5]])
+def test_sum_squares_of_tensors_with_fewer_or_more_counts(counts, monkeypatch):
+    """Two tensors and another number of counts: refused, no tensor is left out of the sum."""
+    from rccl_amd import nccl
+    monkeypatch.setattr(nccl, "_TORCH", {ra.ncclFloat32: "float32"})
+    monkeypatch.setattr(nccl, "_current_device", lambda: 0)
+    called = []
+    monkeypatch.setattr(nccl.lib(), "rcclAmdSumSquares", lambda *a: called.append(a) or 0)
+    call = lambda counts: ra.sum_squares([_Tensor(5, "float32")] * 2, counts, ra.ncclFloat32, P, P, stream=0)  # noqa: E731
+    _refused(lambda: call(counts), "2 tensors with other counts")
+    assert not called
+    call([5, 5]), call(None)
+    assert [a[2] for a in called] == [2, 2]
+
+
 def test_expert_sort_refusals():
     ok = dict(experts=P, expert_type=ra.ncclInt32, tokens=100, topk=8, first_expert=0, n_experts=16, row_align=1, position=P, source=P, offsets=P, counts=P, workspace=None, stream=0)
     for kw, text in ((dict(expert_type=ra.ncclFloat32), "expert type"), (dict(topk=0), "topk"), (dict(topk=65), "topk"), (dict(n_experts=0), "experts"), (dict(n_experts=1025), "experts"),
