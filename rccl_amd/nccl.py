@@ -564,7 +564,7 @@ def sum_squares(tensors, counts, datatype, out, workspace, accumulate=False, str
         if rc >= 0:
             return _check(rc, where)
     own = isinstance(tensors, (list, tuple)) and tensors and hasattr(tensors[0], "data_ptr")
-    if own and counts is None:
+    if counts is None and (own or len(tensors) == 0):
         counts = [t.numel() for t in tensors]
     if counts is None or len(counts) != len(tensors):
         _refuse(where, f"{len(tensors)} tensors with other counts")

@@ -370,6 +370,16 @@ def test_sum_squares(dtype, shift):
         assert float(out) == first + first
 
 
+def test_sum_squares_of_no_tensors_is_zero():
+    import torch
+    import rccl_amd as ra
+    out = torch.full((1,), 7.0, dtype=torch.float64, device="cuda")
+    ra.sum_squares([], None, ra.ncclBfloat16, out, None, accumulate=True)
+    assert float(out) == 7.0
+    ra.sum_squares([], None, ra.ncclBfloat16, out, None)
+    assert float(out) == 0.0
+
+
 def test_sum_squares_past_32_bits_of_elements():
     import torch
     import rccl_amd as ra

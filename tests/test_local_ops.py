@@ -116,6 +116,17 @@ def test_sum_squares_of_tensors_with_fewer_or_more_counts(counts, monkeypatch):
     assert [a[2] for a in called] == [2, 2]
 
 
+def test_sum_squares_of_no_tensors(monkeypatch):
+    """A rank without tensors: its list is empty, and so need not be accompanied by counts."""
+    from rccl_amd import nccl
+    called = []
+    monkeypatch.setattr(nccl.lib(), "rcclAmdSumSquares", lambda *a: called.append(a) or 0)
+    for counts in (None, [], np.zeros(0, dtype=np.int64)):
+        ra.sum_squares([], counts, ra.ncclFloat32, P, None, stream=0)
+    assert [a[:3] for a in called] == [(None, None, 0)] * 3
+    _refused(lambda: ra.sum_squares(np.array([P]), None, ra.ncclFloat32, P, P, stream=0), "counts")
+
+
 def test_expert_sort_refusals():
     ok = dict(experts=P, expert_type=ra.ncclInt32, tokens=100, topk=8, first_expert=0, n_experts=16, row_align=1, position=P, source=P, offsets=P, counts=P, workspace=None, stream=0)
     for kw, text in ((dict(expert_type=ra.ncclFloat32), "expert type"), (dict(topk=0), "topk"), (dict(topk=65), "topk"), (dict(n_experts=0), "experts"), (dict(n_experts=1025), "experts"),
