@@ -44,6 +44,12 @@ def test_adamw_refuses_an_eps_that_fp32_does_not_hold_as_a_normal_number(eps):
     _refused(lambda: _adamw(eps=eps), "normal fp32")
 
 
+@pytest.mark.parametrize("eps", [2.0 ** 128, 1e39, 1.7e308])
+@pytest.mark.parametrize("state_type", [0, 1])
+def test_adamw_refuses_an_eps_that_is_infinite_in_fp32(eps, state_type):
+    _refused(lambda: _adamw(eps=eps, state_type=state_type, rows=[[P, P, P, P, P * state_type, P * state_type, 0, 100]]), "normal fp32")
+
+
 @pytest.mark.parametrize("scales", [(P, P), (P, 0), (0, P)])
 @pytest.mark.parametrize("ntensors", [1, 200])
 def test_adamw_refuses_8_bit_moments_as_floats(scales, ntensors):
