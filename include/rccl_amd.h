@@ -325,7 +325,8 @@ typedef struct {
  * 8-bit float in an update, and rounding to nearest would leave it where it is.  The random bits are a hash of (seed,
  * step, place of the tensor in the call, index of the element), so a step can be repeated exactly.  A sqrt(v) over zero is
  * never rounded to zero.  A moment that is not finite becomes NaN and does not count for its block's scale.
- * eps is 0 or a normal fp32 number.  copyType is ignored where every copy is NULL.  tensors is host memory, read before the
+ * eps is 0 or a normal fp32 number, with 8-bit states at most 2^126 (there the quotient is a product with a reciprocal that is
+ * off by at most one unit of its last place in fp32).  copyType is ignored where every copy is NULL.  tensors is host memory, read before the
  * call returns.  Tensors may not overlap one another. */
 ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntensors, ncclDataType_t paramType, ncclDataType_t gradType,
                           ncclDataType_t copyType, rcclAmdStateType_t stateType, const rcclAmdAdamWConfig_t* config,

@@ -161,8 +161,10 @@ template <typename P, typename G, bool MX> struct Row {
   }
   // Square roots are the correctly rounded ones and nothing is contracted, so that a rounding of an 8-bit state does not depend
   // on how this is compiled.  So is the quotient with fp32 states; with 8-bit states, where VALU time counts, it is a product
-  // with the reciprocal instruction's result, which is off by at most one unit of the last place.  The divisor is zero or
-  // above 2^-75 (a root of an fp32 number), far from where that instruction loses range.
+  // with the reciprocal instruction's result, which is off by at most one unit of the last place.  That instruction takes
+  // subnormal numbers for zero and gives none.  The divisor is zero or from 2^-126 to 2^126: with eps = 0 a root of an fp32
+  // number, 2^-75 at least; otherwise eps, which the host holds to that range, or more by a root of at most 2^64 and its
+  // correction of at most 2^27, which next to 2^126 is rounded away.  (Where g^2 is infinite, so is the divisor, and its reciprocal 0.)
   template <bool WHOLE> __device__ __forceinline__ void update(const Scalars& s, size_t at, int left, uint32_t key) {
     f32x4 r;
     if constexpr (MX) { fm = decode4(qm, xm); r = decode4(qv, xv); fv = r * r; }

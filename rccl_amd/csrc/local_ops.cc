@@ -81,6 +81,8 @@ RA_API ncclResult_t rcclAmdAdamW(const rcclAmdAdamWTensor_t* tensors, int ntenso
   if (!isfinite(c.lr) || !isfinite(c.weightDecay) || !isfinite(c.gradScale) || !isfinite(c.eps) || c.eps < 0.0 || c.gradScale < 0.0)
     RA_REFUSE("%s: lr, weightDecay, gradScale and eps must be finite, gradScale and eps not negative", fn);
   if ((c.eps > 0.0 && c.eps < FLT_MIN) || c.eps > FLT_MAX) RA_REFUSE("%s: eps %g is %s normal fp32 number", fn, c.eps, c.eps < 1.0 ? "below the smallest" : "above the largest");
+  // (the kernel of the 8-bit states multiplies with the divisor's reciprocal, which has to be a normal number too)
+  if (stateType == rcclAmdStateMx8 && c.eps > 0x1p126) RA_REFUSE("%s: eps %g is above 2^126, the largest with 8-bit states", fn, c.eps);
   if (!(c.beta1 >= 0.0 && c.beta1 < 1.0 && c.beta2 >= 0.0 && c.beta2 < 1.0)) RA_REFUSE("%s: beta1 = %g, beta2 = %g outside 0 <= beta < 1", fn, c.beta1, c.beta2);
   if (!c.stepPtr && c.step < 1) RA_REFUSE("%s: step %lld: the first step is 1", fn, (long long)c.step);
   if (c.sumSq && !(c.maxNorm >= 0.0)) RA_REFUSE("%s: maxNorm %g with sumSq", fn, c.maxNorm);

@@ -342,6 +342,26 @@ def test_8_bit_states_past_32_bits_of_elements():
     assert not m[4096:at].any() and not p[4096:at].any()
 
 
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -126, 1e-30, 2.0 ** -75, 1.0, 2.0 ** 126])
+def test_8_bit_states_divided_by_eps_alone(eps):
+    """The divisor is eps, from one end of its range to the other: gradients whose squares vanish in fp32, or are next to
+    nothing beside 2^126 (and large enough for the quotient to be a normal number)."""
+    case = Case([5000], "f32", "f32", None, mx=True, seed=23)
+    case.grad.mul_(1e-22), case.param.zero_()
+    case.cut(case.grad, 0)[::7] = 0
+    for b in (case.m, case.v, case.ms, case.vs):
+        b.zero_()
+    if eps == 2.0 ** 126:
+        case.grad.mul_(1e38).clamp_(-1e16, 1e16)
+    before = case.snapshot()
+    case.run(eps=eps, step=1, seed=6)
+    if eps == 0.0:
+        g, p = case.cut(case.grad, 0), case.cut(case.param, 0)
+        assert (p[g > 0] == -float("inf")).all() and (p[g < 0] == float("inf")).all() and p[g == 0].isnan().all()
+        return
+    _check_mx(case, before, 1.0, 6, eps=eps, step=1)
+
+
 # ------------------------------------------------------------------ norm, clipping, skipping, device scalars
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("shift", [0, 1])

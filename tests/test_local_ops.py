@@ -50,6 +50,12 @@ def test_adamw_refuses_an_eps_that_is_infinite_in_fp32(eps, state_type):
     _refused(lambda: _adamw(eps=eps, state_type=state_type, rows=[[P, P, P, P, P * state_type, P * state_type, 0, 100]]), "normal fp32")
 
 
+@pytest.mark.parametrize("eps", [2.0 ** 127, 3e38, float(np.nextafter(2.0 ** 126, np.inf))])
+def test_adamw_refuses_an_eps_without_a_normal_reciprocal_for_8_bit_states(eps):
+    _refused(lambda: _adamw(eps=eps, state_type=1), "2^126")
+    _refused(lambda: _adamw(eps=eps, rows=[[0, P, P, P, 0, 0, 0, 1]]), "null buffer")      # 32-bit states: eps is taken, the row is not
+
+
 @pytest.mark.parametrize("scales", [(P, P), (P, 0), (0, P)])
 @pytest.mark.parametrize("ntensors", [1, 200])
 def test_adamw_refuses_8_bit_moments_as_floats(scales, ntensors):
