@@ -288,7 +288,9 @@ ncclResult_t rcclAmdNoAllocAsyncError(int device, ncclResult_t* asyncError);
 /* How AdamW's two moments are held.  rcclAmdStateF32: expAvg = m and expAvgSq = v as floats.
  * rcclAmdStateMx8: expAvg holds m and expAvgSq holds sqrt(v) in OCP MX blocks: each 32 consecutive elements of a tensor
  * (the last block may be shorter) are OCP e4m3 bytes (torch.float8_e4m3fn; not the encoding of ncclFp8E4M3) and share one
- * scale byte X with the value 2^(X-127) in expAvgScale / expAvgSqScale.  All zero bytes are the initial state. */
+ * scale byte X in expAvgScale / expAvgSqScale.  X stands for 2^(X-127) from 0 to 254 and for NaN at 255, as in OCP MX; an element
+ * past the largest fp32 number is infinite.  A step writes 1 .. 247 only.  All zero bytes (elements of value 0) are the
+ * initial state. */
 typedef enum { rcclAmdStateF32 = 0, rcclAmdStateMx8 = 1 } rcclAmdStateType_t;
 #define RCCL_AMD_STATE_BLOCK 32
 

@@ -73,7 +73,8 @@ static __device__ __forceinline__ double powN(double x, int64_t n) {
 struct Scalars { float b1, omb1, b2, omb2, eps, decay, stepSize, rootC2, coef; };
 
 // ------------------------------------------------------------------ 8-bit states
-static __device__ __forceinline__ float powerOf(uint32_t scale) { return __uint_as_float(scale << 23); }      // 2^(X-127)
+// 2^(X-127), for the scaled conversions: they take the exponent field of their scale alone, and for them 0 is 2^-127 and 255 NaN.
+static __device__ __forceinline__ float powerOf(uint32_t scale) { return __uint_as_float(scale << 23); }
 static __device__ __forceinline__ f32x4 decode4(uint32_t code, uint32_t scale) {
   const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, powerOf(scale), false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, powerOf(scale), true);
   return f32x4{lo[0], lo[1], hi[0], hi[1]};

@@ -342,6 +342,36 @@ def test_8_bit_states_past_32_bits_of_elements():
     assert not m[4096:at].any() and not p[4096:at].any()
 
 
+def test_8_bit_states_at_every_scale_byte():
+    """Every code with every scale byte X is the code's value times 2^(X-127), as an fp32 number (past its largest: infinite),
+    and NaN where X is 255.  With p = 0, no gradient, v = 0, eps = 1, beta1 = lr = 0.5 the step is p = -m0 / 2: of halvings and
+    products with 1, all exact but for the reciprocal of 1, which may be off by one unit of its last place (2^-23 of the value)."""
+    import torch
+    case = Case([65536], "f32", "f32", None, mx=True)
+    case.grad.zero_(), case.param.zero_(), case.v.zero_(), case.vs.zero_()
+    code = np.tile(np.arange(256, dtype=np.uint8), 256)
+    scale = np.repeat(np.arange(256, dtype=np.uint8), 8)
+    case.cut(case.m, 0).copy_(torch.from_numpy(code).cuda())
+    case.cut_scale(case.ms, 0).copy_(torch.from_numpy(scale).cuda())
+    before = case.snapshot()
+    case.run(lr=0.5, beta1=0.5, beta2=0.5, eps=1.0, weight_decay=0.0, step=1, seed=9)
+    with np.errstate(all="ignore"):
+        m0 = (ref.E4M3[code] * 2.0 ** (np.repeat(scale, 32).astype(np.float64) - 127)).astype(np.float32)
+        m0[np.repeat(scale, 32) == 255] = np.nan
+        m = np.float32(0.5) * m0 + np.float32(0.0)                 # (-0 + 0 is 0)
+    p = _np(case.cut(case.param, 0))
+    fine = np.isfinite(m)
+    assert np.array_equal(np.isnan(p), np.isnan(m)) and np.array_equal(p[np.isinf(m)], -m[np.isinf(m)].astype(np.float64))
+    assert np.all(np.abs(p[fine] + m[fine]) <= 2.0 ** -23 * np.abs(m[fine].astype(np.float64)) + 2.0 ** -149 * (np.abs(m[fine]) < 2.0 ** -126))
+    bits = ref.hash32(9, 1, 0, np.arange(code.size, dtype=np.uint64))
+    want, new = ref.mx_encode(m, (bits & np.uint64(0xFFFF)).astype(np.int64), False)
+    got = _np(case.cut(case.m, 0))
+    assert np.array_equal(_np(case.cut_scale(case.ms, 0)), new)
+    assert np.array_equal(got[fine], want[fine]) and np.all((got[~fine] & 0x7F) == 0x7F)
+    assert not _np(case.cut(case.v, 0)).any()
+    case.untouched(before)
+
+
 @pytest.mark.parametrize("eps", [0.0, 2.0 ** -126, 1e-30, 2.0 ** -75, 1.0, 2.0 ** 126])
 def test_8_bit_states_divided_by_eps_alone(eps):
     """The divisor is eps, from one end of its range to the other: gradients whose squares vanish in fp32, or are next to
