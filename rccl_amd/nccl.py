@@ -398,13 +398,24 @@ def _torch():
                    ncclInt32: torch.int32, ncclInt64: torch.int64})
 
 
+class _NoMirror:
+    """In the place of a CPython module that is not there: no call is plain."""
+    def __getattr__(self, name):
+        return lambda *args: -1
+
+
 def _bind():
-    """The CPython module, with torch's types and the addresses of the library's functions."""
+    """The CPython module, with torch's types and the addresses of the library's functions.  It is built for one interpreter, and
+    not at all without CPython's headers: without it all calls take the way through ctypes."""
     global _mirror
     try:
         from . import _mirror as module
     except ImportError as e:
-        raise OSError(f"the module _mirror is missing ({e}): build it with `make -C rccl_amd/csrc -j8`") from e
+        import warnings
+        warnings.warn(f"rccl_amd: the module _mirror cannot be loaded ({e}); calls of the local operators take a few microseconds more "
+                      "(`make -C rccl_amd/csrc PYTHON=...` builds it)", RuntimeWarning, stacklevel=3)
+        _mirror = _NoMirror()
+        return _mirror
     if not _TORCH:
         _torch()
     L = lib()

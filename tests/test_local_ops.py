@@ -187,3 +187,29 @@ def test_the_mirror_module_leaves_what_is_not_plain():
     for args in ((), ({}, None, None, ()), ({}, None, None, (1,) * 7), ({}, None, None, ("x",) * 8), ({}, None, None, (0,) * 8), ([], None, None, (1,) * 8)):
         with pytest.raises((TypeError, ValueError)):
             m.bind(*args)
+
+
+def test_without_the_mirror_module_calls_take_the_long_way(monkeypatch):
+    """An interpreter that the module was not built for: one warning, and every call reaches the library's own checks."""
+    import sys
+    import types
+    import warnings
+    from rccl_amd import nccl
+    monkeypatch.setitem(sys.modules, "rccl_amd._mirror", None)               # (an import of it fails)
+    monkeypatch.delattr(ra, "_mirror", raising=False)
+    monkeypatch.setattr(nccl, "_mirror", None)
+    s = types.SimpleNamespace(cuda_stream=0)
+    row = np.array([[P, P, P, P, 0, 0, 0, 100]], dtype=np.int64)
+    calls = [lambda: ra.adamw(row, ra.ncclFloat32, ra.ncclFloat32, lr=1e-3, step=0, stream=s),
+             lambda: ra.sum_squares(np.array([P]), np.array([5]), ra.ncclInt32, P, P, stream=s),
+             lambda: ra.expert_sort(P, ra.ncclInt32, 10, 65, 0, 16, 1, P, stream=s),
+             lambda: ra.expert_dispatch(P, P, 64, ra.ncclFloat32, 8, 8, 128, P, stream=s),
+             lambda: ra.expert_combine(P, 64, None, -1, P, ra.ncclFloat32, 8, 8, 128, P, stream=s),
+             lambda: ra.expert_combine_backward(P, 2 * P, 64, P, ra.ncclFloat32, P, 2 * P, ra.ncclFloat32, 8, 8, 128, P, stream=s)]
+    with pytest.warns(RuntimeWarning, match="_mirror"):
+        _refused(calls[0], "first step")
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        for call, text in zip(calls, ("first step", "type", "topk", "same", "same", "overlaps")):
+            _refused(call, text)
+        assert ra.sum_squares_bytes(0) == 0 and ra.expert_sort_bytes(100000, 8, 128) >= 128 * 4
