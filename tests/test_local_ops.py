@@ -1,6 +1,9 @@
 """Argument checks and host logic of the local operators (no GPU: every call here is refused before anything is launched,
 or has nothing to do)."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -191,7 +194,6 @@ def test_the_mirror_module_leaves_what_is_not_plain():
 
 def test_without_the_mirror_module_calls_take_the_long_way(monkeypatch):
     """An interpreter that the module was not built for: one warning, and every call reaches the library's own checks."""
-    import sys
     import types
     import warnings
     from rccl_amd import nccl
@@ -213,3 +215,23 @@ def test_without_the_mirror_module_calls_take_the_long_way(monkeypatch):
         for call, text in zip(calls, ("first step", "type", "topk", "same", "same", "overlaps")):
             _refused(call, text)
         assert ra.sum_squares_bytes(0) == 0 and ra.expert_sort_bytes(100000, 8, 128) >= 128 * 4
+
+
+def _make(tmp_path, python):
+    """What make would run for a build from nothing."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rccl_amd", "csrc")
+    r = subprocess.run(["make", "-n", "-C", csrc, f"PYTHON={python}", f"OUT={tmp_path}/lib.so", f"BUILD={tmp_path}/build"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    assert f"-o {tmp_path}/lib.so" in r.stdout
+    return r.stdout
+
+
+def test_the_library_is_built_without_python(tmp_path):
+    """A host without an interpreter, or with one that has no headers, builds the library alone; others build the module too."""
+    bare = tmp_path / "python"
+    bare.write_text(f"#!/bin/sh\necho {tmp_path}/include\n")
+    bare.chmod(0o755)
+    for python in (str(tmp_path / "nothing"), str(bare)):
+        out = _make(tmp_path, python)
+        assert "without the module" in out and "mirror.c" not in out
+    assert "without the module" not in _make(tmp_path, sys.executable)
