@@ -293,7 +293,8 @@ struct RaSlots {
 // waits for the stores of the first, and with 64 slots in any case 16384 tokens of 8 slots, rows of 8 KiB, take 245 us, with 8 216.
 // More where a rank holds few of the experts and most slots are dropped, so that a wave does not live for one position alone:
 // 65536 tokens of 8 slots, one in eight kept, rows of 8, 4 and 2 KiB 154, 57 and 27 us, a wave for each slot 217, 118
-// and 82 (the gradients 177, 113 and 50 against 312, 291 and 130).  What is kept stands on the device, so the grid fits `rows`
+// and 82 (the gradients 177, 113 and 50 against 312, 291 and 130; one set of inputs again and again, part of which stays in the
+// Infinity Cache).  What is kept stands on the device, so the grid fits `rows`
 // and workgroups too many end at once: that is 40 us of the 154.  half: more slots for a workgroup already where half are dropped
 // (dispatch of 16384 tokens of 8 KiB rows 111 us, not so 132; the gradients 184 and 180).
 static RaSlots slotsOf(const RaRowsArgs& a, int S, bool half) {
@@ -399,7 +400,9 @@ __global__ __launch_bounds__(RA_SLOT_WAVES * 64) RA_FEW_WAVES(S == 1 ? 4 : 8) vo
 #define RA_NARROW_ROWS 2
 // A lane's pack of a narrow row.  The last one ends where the row ends and so repeats elements of the one before it (`twice`), which
 // both lanes read and write alike (the lanes of a row are one wave's: all have read before one writes).  Rows of 100 elements take 25, 28 and 83 us
-// for dispatch, combine and its gradients this way, 39, 47 and 108 with single elements at the end.  !WHOLE: a row shorter than a
+// for dispatch, combine and its gradients this way, 39, 47 and 108 with single elements at the end (524288 slots, one set of inputs
+// again and again; three sets in turn 45, 29 and 82).  Where rows do not end on a cache line the time is up to twice that of rows that
+// do: 128 elements 38, 27 and 54 us, 256 84, 50 and 105, 255 133, 62 and 170.  !WHOLE: a row shorter than a
 // pack, moved element by element.
 template <typename T, bool WHOLE> struct Narrow {
   size_t at; int twice; bool any;
@@ -584,7 +587,7 @@ template <typename T> static __device__ __forceinline__ u32x4 gradients(u32x4 z,
 }
 
 // The gradients of combine.  A wave takes S slots: dz's rows are written while z's rows pass, and their products stay in the
-// wave.  Runs of 8 KiB as in dispatch: half of the slots of 16384 tokens (1.17 to 1.38 GB, as routing goes) 6.0 to 6.1 TB/s, a copy
+// wave.  Runs of 8 KiB as in dispatch: half of the slots of 16384 tokens (1.17 to 1.38 GB, as routing goes) 0.211 to 0.246 ms = 5.5 TB/s, a copy
 // has 6.3; runs of 4 KiB 3 % slower, 2 KiB 5 %; a workgroup for each token, its row in registers, no faster.
 template <typename T, int S>
 __global__ __launch_bounds__(RA_SLOT_WAVES * 64) RA_FEW_WAVES(S == 1 ? 4 : 8) void raLocalKernelCombineBackward(RaSlots n, RaRowsArgs a) {

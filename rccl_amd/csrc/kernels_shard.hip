@@ -212,8 +212,9 @@ __global__ __launch_bounds__(RA_ADAMW_THREADS) __attribute__((amdgpu_waves_per_e
   // stream through one window of memory.  fp32 states: one row for each wave in all, a shard of 67 million elements (1.88 GB) 0.302 ms
   // = 6.2 TB/s; with 2, 4 and 16 rows for each wave 0.313, 0.320 and 0.350, with 32 waves 0.311, with accesses that are not streaming
   // 0.369.  8-bit states: two rows at once and in all (the start of a workgroup counts for more), 33.5 million elements of fp32
-  // (541 MB) 0.089 ms = 6.1 TB/s, of four rows 0.094.  With parameters in 16 bits the 60 VALU cycles for each element count as much
-  // as memory: 32 waves, two rows 0.080 ms (fp16, fp32 gradients, bf16 copy, 477 MB; four rows 0.085), and four rows where nothing but
+  // (541 MB) 0.089 ms = 6.1 TB/s, of four rows 0.094.  With parameters in 16 bits arithmetic is what bounds
+  // it: 66 VALU instructions for each element keep the SIMDs' issue busy for nine tenths of the kernel's cycles (68 and seven tenths with
+  // fp32 parameters).  32 waves, two rows 0.080 ms (fp16, fp32 gradients, bf16 copy, 477 MB; four rows 0.085), and four rows where nothing but
   // 16-bit parameters and gradients is moved beside the states 0.064 (272 MB; two rows 0.067).
   constexpr int U = MX ? 2 : 1;
   constexpr uint32_t STEP = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW;
