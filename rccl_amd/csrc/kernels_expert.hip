@@ -401,8 +401,8 @@ __global__ __launch_bounds__(RA_SLOT_WAVES * 64) RA_FEW_WAVES(S == 1 ? 4 : 8) vo
 // A lane's pack of a narrow row.  The last one ends where the row ends and so repeats elements of the one before it (`twice`), which
 // both lanes read and write alike (the lanes of a row are one wave's: all have read before one writes).  Rows of 100 elements take 25, 28 and 83 us
 // for dispatch, combine and its gradients this way, 39, 47 and 108 with single elements at the end (524288 slots, one set of inputs
-// again and again; three sets in turn 45, 29 and 82).  Where rows do not end on a cache line the time is up to twice that of rows that
-// do: 128 elements 38, 27 and 54 us, 256 84, 50 and 105, 255 133, 62 and 170.  !WHOLE: a row shorter than a
+// again and again; three sets in turn 45, 29 and 82).  Rows that do not end on a cache line take up to twice the time
+// for their bytes: 128 elements 38, 27 and 54 us, 256 84, 50 and 105, 255 133, 62 and 170.  !WHOLE: a row shorter than a
 // pack, moved element by element.
 template <typename T, bool WHOLE> struct Narrow {
   size_t at; int twice; bool any;

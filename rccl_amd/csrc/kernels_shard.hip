@@ -215,7 +215,7 @@ __global__ __launch_bounds__(RA_ADAMW_THREADS) __attribute__((amdgpu_waves_per_e
   // (541 MB) 0.089 ms = 6.1 TB/s, of four rows 0.094.  With parameters in 16 bits arithmetic is what bounds
   // it: 66 VALU instructions for each element keep the SIMDs' issue busy for nine tenths of the kernel's cycles (68 and seven tenths with
   // fp32 parameters).  32 waves, two rows 0.080 ms (fp16, fp32 gradients, bf16 copy, 477 MB; four rows 0.085), and four rows where nothing but
-  // 16-bit parameters and gradients is moved beside the states 0.064 (272 MB; two rows 0.067).
+  // 16-bit parameters and gradients is moved beside the states 0.064 (340 MB; two rows 0.067).
   constexpr int U = MX ? 2 : 1;
   constexpr uint32_t STEP = RA_ADAMW_THREADS / 64 * RA_ADAMW_ROW;
   uint32_t t, chunk0;
